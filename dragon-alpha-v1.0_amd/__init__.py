@@ -10,3 +10,5 @@ from .native import (Cuda_conv3D, Cuda_dconv3D_deltaX, Cuda_dconv3D_deltaW, Cuda
 from . import engine  # noqa: F401,E402
 from . import runtime  # noqa: F401,E402
 from .runtime import Cuda, CudaDevice  # noqa: F401,E402
+from . import dense  # noqa: F401,E402
+from .dense import Cuda_dense  # noqa: F401,E402

@@ -1,0 +1,153 @@
+// Shared declarations of the dense operators (include/alpha_dense.h): activations, the epilogue of a product, the operand
+// description of the tile kernel and the host-side launchers.
+#pragma once
+#include "../../include/alpha_dense.h"
+#include "common.hpp"
+
+namespace alpha {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+// ---- activations ---------------------------------------------------------------------------------------------------
+static __device__ __forceinline__ float dense_act(int act, float z, float k)
+{
+    switch (act) {   // uniform
+    case ALPHA_DENSE_ACT_LEAKY_RELU: return z > 0.f ? z : z * k;
+    case ALPHA_DENSE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case ALPHA_DENSE_ACT_SILU: return z / (1.f + expf(-z));
+    case ALPHA_DENSE_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
+    default: return z;
+    }
+}
+
+static __device__ __forceinline__ float dense_act_slope(int act, float z, float k)
+{
+    switch (act) {
+    case ALPHA_DENSE_ACT_LEAKY_RELU: return z > 0.f ? 1.f : k;
+    case ALPHA_DENSE_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case ALPHA_DENSE_ACT_SILU: {
+        const float s = 1.f / (1.f + expf(-z));
+        return s * (1.f + z * (1.f - s));
+    }
+    case ALPHA_DENSE_ACT_SIGMOID: {
+        const float s = 1.f / (1.f + expf(-z));
+        return s * (1.f - s);
+    }
+    default: return 1.f;
+    }
+}
+
+// ---- element types -------------------------------------------------------------------------------------------------
+template <typename T> static __device__ __forceinline__ float dense_load(const T *p) { return (float)*p; }
+template <typename T> static __device__ __forceinline__ void dense_store(T *p, float v) { *p = (T)v; }   // round to nearest even
+
+// Four consecutive elements; VEC: the address is aligned to the whole group.
+template <typename T> struct Quad;
+template <> struct Quad<float> { typedef floatx4 type; };
+template <> struct Quad<__bf16> { typedef bf16x4 type; };
+
+template <typename T>
+static __device__ __forceinline__ floatx4 quad_load(const T *p)
+{
+    const typename Quad<T>::type v = *reinterpret_cast<const typename Quad<T>::type *>(p);
+    return floatx4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+template <typename T>
+static __device__ __forceinline__ void quad_store(T *p, floatx4 v)
+{
+    typename Quad<T>::type q;
+    q[0] = (T)v[0]; q[1] = (T)v[1]; q[2] = (T)v[2]; q[3] = (T)v[3];
+    *reinterpret_cast<typename Quad<T>::type *>(p) = q;
+}
+
+// ---- three-part split of an fp32 value -----------------------------------------------------------------------------
+// x = h + m + l exactly, each part a bf16 (8 significant bits, round to nearest, signs of the parts their own): 24 bits in
+// all. Where rounding up would leave bf16's range h is truncated; an infinity or NaN is h alone.
+static __device__ __forceinline__ void dense_split(float x, __bf16 &h, __bf16 &m, __bf16 &l)
+{
+    h = (__bf16)x;
+    const uint32_t bits = __float_as_uint(x);
+    if ((bits & 0x7fffffffu) >= 0x7f7f8000u) {
+        if ((bits & 0x7f800000u) == 0x7f800000u) {   // infinity or NaN
+            m = l = (__bf16)0.f;
+            return;
+        }
+        h = (__bf16)__uint_as_float(bits & 0xffff0000u);
+    }
+    const float r = x - (float)h;
+    m = (__bf16)r;
+    l = (__bf16)(r - (float)m);
+}
+
+// ---- the product's epilogue ----------------------------------------------------------------------------------------
+// Plain:  z = acc + bias[n];  Z = z;  Y = act(z) + R     (two stacked products, row2 > 0: rows m < rows1 to Y, m >= row2 to Y2)
+// Gated:  g = acc_g + bias[n], u = acc_u + bias2[n];  Z = g, Z2 = u;  Y = act(g) * u
+struct DenseEpilogue {
+    const void *bias, *bias2, *R;
+    void *Z, *Z2, *Y, *Y2;
+    long ldR, ldZ, ldZ2, ldY, ldY2;
+    int act;
+    float slope;
+    int rows1, row2;
+    int vec;      // groups of four columns are aligned (bases and strides): vector accesses
+};
+
+// C[m, n] = sum over sources and k of A(m, k) B(n, k). An operand of the tile kernel is bf16; an fp32 tensor comes as
+// three of them (dense_split), `plane` elements apart.
+struct DenseOperand {
+    const __bf16 *p[2];   // up to two sources
+    long ld;              // element (row r, column c) at r * ld + c
+    long plane;
+};
+struct DenseProduct {
+    DenseOperand A, B;
+    int parts;            // 1, or 3 (fp32: six of the nine products of parts)
+    int sources;          // 2: the sum goes on over A.p[1], B.p[1]
+    int gated;            // B.p[0], B.p[1] are the two filters of a gated pair
+    int a_t, b_t;         // operand stored with k as its rows
+    int M, N;             // N: of one filter where gated
+    int K;
+    int f32;              // output type
+    DenseEpilogue ep;
+    float *partial;       // room for partial sums, `partial_bytes`
+    size_t partial_bytes;
+};
+size_t dense_product_partial_bytes(int M, int N, int K, int parts, int sources, int gated);
+hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p);
+
+// Few rows, operands as they are (dense_few_rows.hip).
+struct DenseFewRows {
+    const void *X, *W, *W2;
+    long ldX, ldW, ldW2;
+    int f32, gated;
+    int M, N, K;
+    DenseEpilogue ep;
+};
+
+// dst planes <- src[rows, cols]: fp32 in three parts, bf16 as it is; row stride ld (multiple of 8), columns cols .. ld zero.
+hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, __bf16 *dst, long ld, long plane);
+
+// deltaZ (or deltaG and deltaU) as packed planes and the column sums of the unrounded values.
+struct DenseDelta {
+    const void *dY, *Z, *U;
+    long ldY, ldZ, ldU;
+    int f32, act, gated;
+    float slope;
+    long rows;
+    int cols;
+    __bf16 *dst, *dst2;   // NULL: only the sums
+    long ld;              // columns written (cols, then zeros): a multiple of 8
+    long ld2, plane;      // row stride of dst, dst2
+    void *dB, *dB2;       // NULL: no sums
+    float *sums;          // dense_delta_sum_bytes of scratch
+};
+size_t dense_delta_sum_bytes(long rows, int cols, int gated);
+hipError_t launch_dense_delta(hipStream_t s, const DenseDelta &d);
+
+// Clipping by the global norm (grad_clip.hip); `words`: the sum of grad_pieces over the tensors.
+long grad_pieces(long length);
+hipError_t launch_grad_clip(hipStream_t s, int count, const int *types, const int64_t *lengths, const void *const *src, void *const *dst,
+                            float max_norm, float eps, float *norm_c, double *words);
+
+}  // namespace alpha

@@ -1,0 +1,11 @@
+// The tile kernel for the gated pair of products (forward).
+#include "dense_gemm_launch.hpp"
+
+namespace alpha {
+
+hipError_t launch_dense_tile_gated(hipStream_t s, const DenseTileArgs &a, bool big, int f32)
+{
+    return launch_dense_tile_any<false, false, DENSE_GATED, DENSE_PARTIAL_GATED>(s, a, big, f32);
+}
+
+}  // namespace alpha

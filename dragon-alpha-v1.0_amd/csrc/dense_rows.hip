@@ -1,0 +1,202 @@
+// The passes around a dense product, each bound by memory: operands made ready for the tile kernel (three-part split of
+// fp32, rows of bf16 that the 128-bit loads cannot take copied to ones they can), and deltaZ = deltaY * act'(Z) with its
+// column sums.
+#include "dense_common.hpp"
+
+#include <algorithm>
+
+namespace alpha {
+
+namespace {
+
+// Eight consecutive elements of a row, c .. c+7 of `cols`; the rest zeros. VEC: 16-byte loads are possible.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *row, int c, int cols, float (&v)[8])
+{
+    if (VEC && c + 8 <= cols) {
+        const floatx4 lo = quad_load(row + c), hi = quad_load(row + c + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = lo[e], v[4 + e] = hi[e];
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = c + e < cols ? dense_load(row + c + e) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_parts(__bf16 *dst, long plane, const float (&v)[8])
+{
+    bf16x8 h, m, l;
+    if constexpr (__is_same(T, float)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            __bf16 x, y, z;
+            dense_split(v[e], x, y, z);
+            h[e] = x, m[e] = y, l[e] = z;
+        }
+        *reinterpret_cast<bf16x8 *>(dst + plane) = m;
+        *reinterpret_cast<bf16x8 *>(dst + 2 * plane) = l;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = (__bf16)v[e];
+    }
+    *reinterpret_cast<bf16x8 *>(dst) = h;
+}
+
+}  // namespace
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dense_pack_kernel(const T *__restrict__ src, long src_ld, long total, int cols, __bf16 *__restrict__ dst,
+                                                         long ld, long plane, FastDiv d_chunks)
+{
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long row = fdiv((uint32_t)i, d_chunks);
+        const int c = (int)(i - row * d_chunks.d) * 8;
+        float v[8];
+        load8<T, VEC>(src + row * src_ld, c, cols, v);
+        store_parts<T>(dst + row * ld + c, plane, v);
+    }
+}
+
+hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, __bf16 *dst, long ld, long plane)
+{
+    const long chunks = ld / 8, total = rows * chunks;
+    if (total <= 0) return hipSuccess;
+    if (total >= (1l << 31)) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)std::min<long>((total + 255) / 256, 16384));
+    const FastDiv d = make_fastdiv((uint32_t)chunks);
+    const bool vec = (reinterpret_cast<uintptr_t>(src) & (f32 ? 15 : 7)) == 0 && (src_ld & 3) == 0;
+    if (f32) {
+        const float *p = static_cast<const float *>(src);
+        if (vec) hipLaunchKernelGGL((dense_pack_kernel<float, true>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
+        else hipLaunchKernelGGL((dense_pack_kernel<float, false>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
+    } else {
+        const __bf16 *p = static_cast<const __bf16 *>(src);
+        if (vec) hipLaunchKernelGGL((dense_pack_kernel<__bf16, true>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
+        else hipLaunchKernelGGL((dense_pack_kernel<__bf16, false>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
+    }
+    return hipGetLastError();
+}
+
+// A workgroup takes 256 columns (32 lanes of 8) of a run of rows, eight rows at a time; its column sums go to sums[run].
+template <typename T, bool VEC, bool GATED>
+__global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, long rows_per)
+{
+    __shared__ float part[GATED ? 2 : 1][8][257];
+    const int lane = threadIdx.x & 31, ry = threadIdx.x >> 5, c = (blockIdx.x * 32 + lane) * 8;
+    const long r0 = (long)blockIdx.y * rows_per, r1 = r0 + rows_per < d.rows ? r0 + rows_per : d.rows;
+    float sum[8], sum2[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum[e] = sum2[e] = 0.f;
+    if (c < d.ld) {
+        for (long r = r0 + ry; r < r1; r += 8) {
+            float dy[8], z[8], u[8], out2[8];
+            load8<T, VEC>(static_cast<const T *>(d.dY) + r * d.ldY, c, d.cols, dy);
+            if (GATED || d.act != ALPHA_DENSE_ACT_NONE) load8<T, VEC>(static_cast<const T *>(d.Z) + r * d.ldZ, c, d.cols, z);
+            if constexpr (GATED) load8<T, VEC>(static_cast<const T *>(d.U) + r * d.ldU, c, d.cols, u);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (c + e >= d.cols) {   // pad columns: zeros, whatever act(0) is
+                    dy[e] = out2[e] = 0.f;
+                } else if constexpr (GATED) {
+                    out2[e] = dy[e] * dense_act(d.act, z[e], d.slope);
+                    dy[e] *= u[e] * dense_act_slope(d.act, z[e], d.slope);
+                } else if (d.act != ALPHA_DENSE_ACT_NONE) {
+                    dy[e] *= dense_act_slope(d.act, z[e], d.slope);
+                }
+                sum[e] += dy[e];
+                if constexpr (GATED) sum2[e] += out2[e];
+            }
+            if (d.dst) store_parts<T>(d.dst + r * d.ld2 + c, d.plane, dy);
+            if constexpr (GATED)
+                if (d.dst2) store_parts<T>(d.dst2 + r * d.ld2 + c, d.plane, out2);
+        }
+    }
+    if (!d.sums) return;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        part[0][ry][lane * 8 + e] = sum[e];
+        if constexpr (GATED) part[1][ry][lane * 8 + e] = sum2[e];
+    }
+    __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= d.cols) return;
+#pragma unroll
+    for (int w = 0; w < (GATED ? 2 : 1); w++) {
+        float t = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; y++) t += part[w][y][threadIdx.x];
+        d.sums[((long)blockIdx.y * (GATED ? 2 : 1) + w) * d.cols + col] = t;
+    }
+}
+
+// dB[col] = sum over the runs, in a fixed order: 16 lanes a column, each its share of the runs.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_delta_sum_kernel(const float *__restrict__ sums, int runs, int cols, int which, int of, T *__restrict__ dB)
+{
+    __shared__ float part[16][17];
+    const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4, col = blockIdx.x * 16 + cx;
+    float t = 0.f;
+    if (col < cols)
+        for (int r = ry; r < runs; r += 16) t += sums[((long)r * of + which) * cols + col];
+    part[ry][cx] = t;
+    __syncthreads();
+    if (ry == 0 && col < cols) {
+        t = 0.f;
+#pragma unroll
+        for (int y = 0; y < 16; y++) t += part[y][cx];
+        dense_store(dB + col, t);
+    }
+}
+
+namespace {
+
+// Runs of rows: enough workgroups for the device, at least 32 rows each (a run costs a row of sums), at most 512 runs.
+long delta_rows_per(long rows, int cols)
+{
+    const long blocks_x = (cols + 255) / 256, want = std::max<long>(1, 2048 / std::max<long>(1, blocks_x));
+    const long runs = std::min<long>(512, std::max<long>(1, std::min(want, rows / 32)));
+    return std::max<long>(1, (rows + runs - 1) / runs);
+}
+
+template <typename T>
+hipError_t launch_delta_typed(hipStream_t s, const DenseDelta &d, bool vec, long rows_per, int runs)
+{
+    const dim3 grid((unsigned)((d.ld + 255) / 256), (unsigned)std::max(runs, 1));
+    if (runs > 0) {
+        if (d.gated) {
+            if (vec) hipLaunchKernelGGL((dense_delta_kernel<T, true, true>), grid, dim3(256), 0, s, d, rows_per);
+            else hipLaunchKernelGGL((dense_delta_kernel<T, false, true>), grid, dim3(256), 0, s, d, rows_per);
+        } else {
+            if (vec) hipLaunchKernelGGL((dense_delta_kernel<T, true, false>), grid, dim3(256), 0, s, d, rows_per);
+            else hipLaunchKernelGGL((dense_delta_kernel<T, false, false>), grid, dim3(256), 0, s, d, rows_per);
+        }
+    }
+    const dim3 cols((unsigned)((d.cols + 15) / 16));
+    const int of = d.gated ? 2 : 1;
+    if (d.dB) hipLaunchKernelGGL((dense_delta_sum_kernel<T>), cols, dim3(256), 0, s, d.sums, runs, d.cols, 0, of, static_cast<T *>(d.dB));
+    if (d.dB2) hipLaunchKernelGGL((dense_delta_sum_kernel<T>), cols, dim3(256), 0, s, d.sums, runs, d.cols, 1, of, static_cast<T *>(d.dB2));
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t dense_delta_sum_bytes(long rows, int cols, int gated)
+{
+    if (rows <= 0 || cols <= 0) return 0;
+    const long per = delta_rows_per(rows, cols), runs = (rows + per - 1) / per;
+    return (size_t)runs * cols * (gated ? 2 : 1) * 4;
+}
+
+hipError_t launch_dense_delta(hipStream_t s, const DenseDelta &given)
+{
+    DenseDelta d = given;
+    if (d.cols <= 0) return hipSuccess;
+    if (!d.dB && !d.dB2) d.sums = nullptr;
+    const long per = delta_rows_per(d.rows, d.cols), runs = d.rows > 0 ? (d.rows + per - 1) / per : 0;
+    auto fits = [&](const void *p, long ld) { return (reinterpret_cast<uintptr_t>(p) & (d.f32 ? 15 : 7)) == 0 && (ld & 3) == 0; };
+    const bool vec = fits(d.dY, d.ldY) && fits(d.Z, d.ldZ) && fits(d.U, d.ldU);
+    return d.f32 ? launch_delta_typed<float>(s, d, vec, per, (int)runs) : launch_delta_typed<__bf16>(s, d, vec, per, (int)runs);
+}
+
+}  // namespace alpha
