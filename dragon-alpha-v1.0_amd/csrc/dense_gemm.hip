@@ -39,8 +39,9 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
                     u[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[1], a.B[1], (n + e) * b_row, b_k, a.planeB, 1, a.K);
             }
         }
-        if constexpr (GATED) dense_finish4_gated<T>(a.ep, v, u, m, n, a.N);
-        else dense_finish4<T>(a.ep, v, m, n, a.N);
+        float x[4] = {v[0], v[1], v[2], v[3]}, y[4] = {u[0], u[1], u[2], u[3]};
+        if constexpr (GATED) dense_finish_gated<T>(a.ep, x, y, m, n, a.N);
+        else dense_finish<T>(a.ep, x, m, n, a.N);
     }
 }
 
@@ -55,7 +56,7 @@ struct Plan {
 Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t room)
 {
     const int cus = std::max(1, device_cu_count());
-    const int nk = std::max(1, (K + 63) / 64), steps = nk * (parts == 3 ? 6 : 1) * sources;
+    const int nk = std::max(1, (K + 31) / 32), steps = nk * (parts == 3 ? 6 : 1) * sources;
     const double out_bytes = (double)M * N * (gated ? 2 : 1) * 4;
     Plan best{};
     double best_us = 1e30;
@@ -65,11 +66,12 @@ Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t ro
         const long tiles = (long)tm * tn, slots = (long)cus * (big ? 1 : 2);
         for (int split = 1; split <= 64; split++) {
             // whole k steps: a piece holds all parts of its products, so none leaves fp32's range that the sum would not
-            const int combos = steps / nk, per = (nk + split - 1) / split * combos;
-            if (split > 1 && (per < 4 || (long)split * M * N * (gated ? 2 : 1) * 4 > (long)room)) break;
+            // (and an even number of steps: the kernel's loop does two at a time)
+            const int combos = steps / nk, per = (nk + 2 * split - 1) / (2 * split) * 2 * combos;
+            if (split > 1 && (per < 8 || (long)split * M * N * (gated ? 2 : 1) * 4 > (long)room)) break;
             if ((steps + per - 1) / per != split) continue;   // every piece has a step
             const long rounds = (tiles * split + slots - 1) / slots;
-            double us = rounds * (per * (big ? 1.3 : 0.75) + 3.0);
+            double us = rounds * (per * (big ? 0.65 : 0.4) + 3.0);
             if (split > 1) us += 3.0 + out_bytes * (split * 2 + 1) / 4e6;
             if (us < best_us) {
                 best_us = us;
@@ -108,7 +110,6 @@ hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
     a.parts6 = p.parts == 3 ? 6 : 1;
     a.combos = a.parts6 * p.sources;
     a.steps = plan.steps;
-    a.nk = plan.steps / a.combos;
     a.split = plan.split;
     a.per = plan.per;
     a.tiles_m = plan.tiles_m;

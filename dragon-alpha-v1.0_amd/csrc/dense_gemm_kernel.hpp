@@ -1,17 +1,19 @@
 // The dense product's tile kernel: C[m, n] = sum_k A(m, k) B(n, k), bf16 operands, fp32 sums, on v_mfma_f32_16x16x32_bf16.
 //
-// A workgroup computes BM x BN of C in steps of 64 k. A step's tiles go from memory straight into LDS (128-bit
-// buffer loads with LDS as their target) two steps ahead into two buffers; a wavefront owns BM/WM x BN/WN of C in
-// registers and reads its operand fragments one half step ahead of the MFMAs that use them, so the one barrier of a step
-// falls between two runs of MFMAs whose operands are in registers already.
+// A workgroup computes BM x BN of C in steps of 32 k. A step's tiles go from memory straight into LDS (128-bit buffer
+// loads with LDS as their target) through a ring of four buffers, four steps ahead; a wavefront owns BM/WM x BN/WN of C in
+// registers and reads the operand fragments of a step while it multiplies those of the step before, so the one barrier of
+// a step falls between two runs of MFMAs whose operands are in registers already.
 // Operands may be stored with k along their rows (row r: k = 0, 1, ..: "straight") or with k as the rows ("T"). Straight
-// tiles are [rows][64 k] of 128-byte rows whose eight 16-byte chunks are permuted by the row (chunk ^ f(row)), so the 16
-// rows that a fragment read touches lie in different banks; T tiles are [64 k][rows] and are read by the transposing LDS
-// load, four k of 16 rows per instruction, their 32-byte pieces permuted by k.
+// tiles are [rows][32 k] of 64-byte rows whose four 16-byte chunks are permuted by the row, so the 16 lanes that LDS serves
+// in a cycle (eight rows, two chunks each) touch different banks; T tiles are [32 k][rows] and are read by the transposing
+// LDS load, four k of 16 rows per instruction, their 32-byte pieces permuted by k.
 // Rows beyond the operand read zeros (the buffer descriptor ends with the last row's last 16-byte chunk: rows are whole
 // chunks long, zeros after their last element); k beyond K reads zeros too.
-// The MFMA's rows are n and its columns m, so a lane holds runs of consecutive n of one m. Straight B: fragment nf of a
-// 64-column group takes the columns 16 * (i / 4) + 4 * nf + i % 4 (i = 0..15), which makes a lane's run 16 long.
+// The MFMA's rows are n and its columns m, so a lane holds four consecutive n of one m. A finished tile goes through LDS
+// (each wavefront its own part) so that every lane then has eight consecutive columns and a row leaves as one run of 128
+// bytes: stored from the registers as they are, 4096 x 4096 of bf16 took 17 us to write, this way 10.
+// Gated: of every 64 tile columns 32 are of one filter and 32, the same ones, of the other.
 #pragma once
 #include "dense_common.hpp"
 
@@ -24,11 +26,10 @@ struct DenseTileArgs {
     const __bf16 *A[2], *B[2];
     long ldA, ldB, planeA, planeB;
     int M, N, K;
-    int nk;            // steps of 64 k
-    int combos;        // products per k step: parts (1 or 6) x sources
+    int combos;        // products per 32 k: parts (1 or 6) x sources
     int parts6;        // 6 for the three-part split, else 1
-    int steps;         // nk * combos
-    int split, per;    // the reduction is cut into `split` runs of `per` steps
+    int steps;         // combos for every 32 k
+    int split, per;    // the reduction is cut into `split` runs of `per` steps (an even number)
     int tiles_m, tiles_n;
     DenseEpilogue ep;
     float *partial;    // [split][M][columns of C]
@@ -45,11 +46,10 @@ static __device__ __forceinline__ void load_to_lds(unsigned lds, unsigned voffse
     asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc) : "memory");
 }
 
-static __device__ __forceinline__ uintx4 make_rsrc(const void *p, long bytes)
+static __device__ __forceinline__ uintx4 make_rsrc(const void *p, unsigned bytes)   // bytes < 2^31: lanes that must read zeros ask for 2^31
 {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
-    const long n = bytes < 0 ? 0 : (bytes > 0x7fffffffl ? 0x7fffffffl : bytes);
-    return uintx4{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, (unsigned)n, 0x00020000u};
+    return uintx4{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 
 // which parts the c-th of the six products multiplies: (l,h) (h,l) (m,m) (m,h) (h,m) (h,h), small ones first
@@ -75,69 +75,170 @@ static __device__ __attribute__((noinline)) float dense_element(const __bf16 *A0
     return acc;
 }
 
-// The plain epilogue of four consecutive columns n .. n+3 of row m (fewer at the right edge).
-template <typename T>
-static __device__ __forceinline__ void dense_finish4(const DenseEpilogue &ep, floatx4 v, long m, int n, int N)
+// R consecutive elements of a row, aligned to groups of four.
+template <int R, typename T>
+static __device__ __forceinline__ void run_load(const T *p, float (&v)[R])
+{
+#pragma unroll
+    for (int i = 0; i < R; i += 4) {
+        const floatx4 q = quad_load(p + i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[i + e] = q[e];
+    }
+}
+template <int R, typename T>
+static __device__ __forceinline__ void run_store(T *p, const float (&v)[R])
+{
+    if constexpr (R == 8 && sizeof(T) == 2) {   // one 128-bit store (the hardware takes 8-byte alignment)
+        bf16x8 q;
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[e] = (T)v[e];
+        __builtin_memcpy(__builtin_assume_aligned(p, 8), &q, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; i += 4) quad_store(p + i, floatx4{v[i], v[i + 1], v[i + 2], v[i + 3]});
+    }
+}
+template <int R>
+static __device__ __forceinline__ void run_act(int act, float (&v)[R], float k)
+{
+    switch (act) {   // one branch for the run
+    case ALPHA_DENSE_ACT_LEAKY_RELU:
+#pragma unroll
+        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_LEAKY_RELU, v[e], k);
+        break;
+    case ALPHA_DENSE_ACT_GELU:
+#pragma unroll
+        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_GELU, v[e], k);
+        break;
+    case ALPHA_DENSE_ACT_SILU:
+#pragma unroll
+        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_SILU, v[e], k);
+        break;
+    case ALPHA_DENSE_ACT_SIGMOID:
+#pragma unroll
+        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_SIGMOID, v[e], k);
+        break;
+    default: break;
+    }
+}
+
+// The epilogues of R consecutive columns n .. n+R-1 of row m (fewer at the right edge).
+template <typename T, int R>
+static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n, int N)
 {
     const bool second = ep.row2 > 0 && m >= ep.row2;
     if (ep.row2 > 0 && !second && m >= ep.rows1) return;   // a row between two stacked products
     T *Y = static_cast<T *>(second ? ep.Y2 : ep.Y) + (second ? (m - ep.row2) * ep.ldY2 : m * ep.ldY) + n;
-    const T *bias = static_cast<const T *>(ep.bias), *R = static_cast<const T *>(ep.R);
+    const T *bias = static_cast<const T *>(ep.bias), *res = static_cast<const T *>(ep.R);
     T *Z = static_cast<T *>(ep.Z);
-    if (ep.vec && n + 4 <= N) {
-        if (bias) v += quad_load(bias + n);
-        if (Z) quad_store(Z + m * ep.ldZ + n, v);
-        if (ep.act != ALPHA_DENSE_ACT_NONE)
-            v = floatx4{dense_act(ep.act, v[0], ep.slope), dense_act(ep.act, v[1], ep.slope), dense_act(ep.act, v[2], ep.slope), dense_act(ep.act, v[3], ep.slope)};
-        if (R) v += quad_load(R + m * ep.ldR + n);
-        quad_store(Y, v);
-        return;
-    }
+    const bool whole = R % 4 == 0 && ep.vec && n + R <= N;
+    float t[R];
+    if (bias) {
+        if constexpr (R % 4 == 0)
+            if (whole) run_load(bias + n, t);
+        if (!whole) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (n + i < N) {
-            float z = v[i];
-            if (bias) z += dense_load(bias + n + i);
-            if (Z) dense_store(Z + m * ep.ldZ + n + i, z);
-            z = dense_act(ep.act, z, ep.slope);
-            if (R) z += dense_load(R + m * ep.ldR + n + i);
-            dense_store(Y + i, z);
+            for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(bias + n + e) : 0.f;
         }
+#pragma unroll
+        for (int e = 0; e < R; e++) v[e] += t[e];
+    }
+    if (Z) {
+        if constexpr (R % 4 == 0)
+            if (whole) run_store(Z + m * ep.ldZ + n, v);
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < R; e++)
+                if (n + e < N) dense_store(Z + m * ep.ldZ + n + e, v[e]);
+        }
+    }
+    run_act(ep.act, v, ep.slope);
+    if (res) {
+        if constexpr (R % 4 == 0)
+            if (whole) run_load(res + m * ep.ldR + n, t);
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(res + m * ep.ldR + n + e) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < R; e++) v[e] += t[e];
+    }
+    if constexpr (R % 4 == 0)
+        if (whole) run_store(Y, v);
+    if (!whole) {
+#pragma unroll
+        for (int e = 0; e < R; e++)
+            if (n + e < N) dense_store(Y + e, v[e]);
+    }
 }
 
-template <typename T>
-static __device__ __forceinline__ void dense_finish4_gated(const DenseEpilogue &ep, floatx4 g, floatx4 u, long m, int n, int N)
+template <typename T, int R>
+static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &ep, float (&g)[R], float (&u)[R], long m, int n, int N)
 {
     T *Y = static_cast<T *>(ep.Y) + m * ep.ldY + n;
-    const T *bg = static_cast<const T *>(ep.bias), *bu = static_cast<const T *>(ep.bias2);
-    T *G = static_cast<T *>(ep.Z), *U = static_cast<T *>(ep.Z2);
-    if (ep.vec && n + 4 <= N) {
-        if (bg) g += quad_load(bg + n);
-        if (bu) u += quad_load(bu + n);
-        if (G) quad_store(G + m * ep.ldZ + n, g);
-        if (U) quad_store(U + m * ep.ldZ2 + n, u);
-        quad_store(Y, floatx4{dense_act(ep.act, g[0], ep.slope), dense_act(ep.act, g[1], ep.slope), dense_act(ep.act, g[2], ep.slope),
-                              dense_act(ep.act, g[3], ep.slope)} * u);
-        return;
-    }
+    const bool whole = R % 4 == 0 && ep.vec && n + R <= N;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (n + i < N) {
-            const float gi = g[i] + (bg ? dense_load(bg + n + i) : 0.f), ui = u[i] + (bu ? dense_load(bu + n + i) : 0.f);
-            if (G) dense_store(G + m * ep.ldZ + n + i, gi);
-            if (U) dense_store(U + m * ep.ldZ2 + n + i, ui);
-            dense_store(Y + i, dense_act(ep.act, gi, ep.slope) * ui);
+    for (int which = 0; which < 2; which++) {
+        float(&v)[R] = which ? u : g;
+        const T *bias = static_cast<const T *>(which ? ep.bias2 : ep.bias);
+        T *Z = static_cast<T *>(which ? ep.Z2 : ep.Z) + m * (which ? ep.ldZ2 : ep.ldZ) + n;
+        if (bias) {
+            float t[R];
+            if constexpr (R % 4 == 0)
+                if (whole) run_load(bias + n, t);
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(bias + n + e) : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < R; e++) v[e] += t[e];
         }
+        if (which ? ep.Z2 != nullptr : ep.Z != nullptr) {
+            if constexpr (R % 4 == 0)
+                if (whole) run_store(Z, v);
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < R; e++)
+                    if (n + e < N) dense_store(Z + e, v[e]);
+            }
+        }
+    }
+    run_act(ep.act, g, ep.slope);
+#pragma unroll
+    for (int e = 0; e < R; e++) g[e] *= u[e];
+    if constexpr (R % 4 == 0)
+        if (whole) run_store(Y, g);
+    if (!whole) {
+#pragma unroll
+        for (int e = 0; e < R; e++)
+            if (n + e < N) dense_store(Y + e, g[e]);
+    }
 }
+
+// Between LDS accesses of one wavefront's lanes: LDS serves a wavefront in order, the compiler must keep that order.
+static __device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Which 16-byte chunk of a T tile's k row a chunk is kept at: number ^ this. The 32 lanes that one cycle of a transposing
+// read serves touch eight k rows (0 .. 3 and 8 .. 11), whose 32-byte pieces so lie in eight different parts of the 256 bytes
+// that a cycle delivers.
+static __device__ __forceinline__ int t_permutation(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
+// The same for a straight tile, by g = row / 4. The 16 lanes that a cycle of a 128-bit read serves are rows 0-3 and 12-15
+// of a fragment in one chunk and rows 4-11 in the chunk beside it (or the other way round); four rows are 256 bytes, so the
+// four groups of rows must come to four different chunks: 0, 3, 2, 1 for g = 0 .. 3. Counted: no conflicts.
+static __device__ __forceinline__ int s_permutation(int g) { return (g & 1) | ((g ^ (g >> 1)) & 1) << 1; }
 
 template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const DenseTileArgs a)
 {
     constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
-    constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT;       // 16-byte loads of a thread per step
-    constexpr unsigned ABYTES = BM * 128, BBYTES = BN * 128, STAGE = ABYTES + BBYTES;
+    constexpr int LA = BM * 4 / NT, LB = BN * 4 / NT;       // 16-byte loads of a thread per step
+    constexpr unsigned ABYTES = BM * 64, BBYTES = BN * 64, STAGE = ABYTES + BBYTES, RING = 4 * STAGE;
     constexpr bool GATED = OUT == DENSE_GATED || OUT == DENSE_PARTIAL_GATED;
-    constexpr bool PERM = !BT;                              // a lane's columns in runs of 16
     static_assert(TM % 16 == 0 && TN % 64 == 0 && LA >= 1 && LB >= 1 && NT % 256 == 0, "tile shape");
     extern __shared__ char smem[];
 
@@ -167,28 +268,26 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     if constexpr (AT) {
 #pragma unroll
         for (int j = 0; j < LA; j++) {
-            const int slot = j * NT + tid, row = slot / (BM / 8), c = (slot % (BM / 8)) ^ ((row & 3) << 1);
+            const int slot = j * NT + tid, row = slot / (BM / 8), c = (slot % (BM / 8)) ^ t_permutation(row);
             offA[j] = (unsigned)((long)row * a.ldA * 2) + c * 16;
         }
     } else {
-        kchunkA = ((lane & 7) ^ (lane >> 3)) * 8;
+        kchunkA = ((lane & 3) ^ s_permutation(lane >> 4)) * 8;    // tile row .. + (lane >> 2)
 #pragma unroll
-        for (int j = 0; j < LA; j++) offA[j] = (unsigned)((long)(j * (NT / 8) + (tid >> 3)) * a.ldA * 2) + kchunkA * 2;
+        for (int j = 0; j < LA; j++) offA[j] = (unsigned)((long)(j * (NT / 4) + (tid >> 2)) * a.ldA * 2) + kchunkA * 2;
     }
     if constexpr (BT) {
 #pragma unroll
         for (int j = 0; j < LB; j++) {
-            const int slot = j * NT + tid, row = slot / (BN / 8), c = (slot % (BN / 8)) ^ ((row & 3) << 1);
+            const int slot = j * NT + tid, row = slot / (BN / 8), c = (slot % (BN / 8)) ^ t_permutation(row);
             offB[j] = (unsigned)((long)row * a.ldB * 2) + c * 16;
         }
     } else {
-        // tile row r; its bank permutation uses bits 0, 1 and 4, the ones that differ within a fragment's 16 rows
-        kchunkB = ((lane & 7) ^ (((lane >> 3) & 3) | (((wave >> 1) & 1) << 2))) * 8;
+        kchunkB = ((lane & 3) ^ s_permutation(lane >> 4)) * 8;
 #pragma unroll
         for (int j = 0; j < LB; j++) {
-            const int r = j * (NT / 8) + (tid >> 3);
-            // gated: of every 16 tile rows the first 8 are the gate's filter, the last 8 the other's (one filter per wavefront's load)
-            const int row = GATED ? (r >> 6) * 32 + ((r >> 4) & 3) * 8 + (r & 7) : r;
+            const int r = j * (NT / 4) + (tid >> 2);
+            const int row = GATED ? (r >> 6) * 32 + (r & 31) : r;   // gated: 32 rows of one filter, 32 of the other
             offB[j] = (unsigned)((long)row * a.ldB * 2) + kchunkB * 2;
         }
     }
@@ -197,87 +296,83 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     const int t0 = piece * a.per;
     int left = a.steps - t0;
     if (left > a.per) left = a.per;
-    int kt = t0 / a.combos, combo = t0 % a.combos;    // of the next step to load
+    int combo = t0 % a.combos;                         // of the next step to load
+    int krem = a.K - t0 / a.combos * 32;               // k from its first on; <= 0: nothing, zeros
+    const long stepA = AT ? 32 * a.ldA : 32, stepB = BT ? 32 * a.ldB : 32;
+    const long atA = AT ? (long)m0 : (long)m0 * a.ldA, atB = BT ? (long)n0 : (long)n0 * a.ldB;
+    const __bf16 *pA = a.A[0] + atA + t0 / a.combos * stepA, *pB = a.B[0] + atB + t0 / a.combos * stepB;   // first source, first part
+    const long toA1 = a.A[1] - a.A[0], toB1 = a.B[1] - a.B[0];
+    // bytes from a tile's first element to its end: straight, its rows' last chunk; T, of one k row
+    const int spanN = GATED ? BN / 2 : BN;
+    const unsigned endA = AT ? (unsigned)((a.M - m0 + 7) & ~7) * 2 : (unsigned)(((long)((a.M - m0 < BM ? a.M - m0 : BM) - 1) * a.ldA + 32) * 2);
+    const unsigned endB = BT ? (unsigned)((a.N - n0 + 7) & ~7) * 2 : (unsigned)(((long)((a.N - n0 < spanN ? a.N - n0 : spanN) - 1) * a.ldB + 32) * 2);
 
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-    auto load_step = [&](unsigned stage) {
-        const int src = combo >= a.parts6 ? 1 : 0, c = combo - src * a.parts6;
-        const int pa = a.parts6 == 6 ? combo_part_a(c) : 0, pb = a.parts6 == 6 ? combo_part_b(c) : 0;
-        const int krem = kt < a.nk ? a.K - kt * 64 : 0;   // beyond the last step: nothing
-        const __bf16 *pA = (src ? a.A[1] : a.A[0]) + pa * a.planeA;
-        const __bf16 *pB = (GATED ? ((wave & 1) ? a.B[1] : a.B[0]) : (src ? a.B[1] : a.B[0])) + pb * a.planeB;
-        long bytesA, bytesB;
-        if constexpr (AT) {
-            pA += (long)kt * 64 * a.ldA + m0;
-            bytesA = krem > 0 ? ((long)(krem - 1) * a.ldA + ((a.M - m0 + 7) & ~7)) * 2 : 0;
-        } else {
-            const int rows = a.M - m0 < BM ? a.M - m0 : BM;
-            pA += (long)m0 * a.ldA + kt * 64;
-            bytesA = krem > 0 ? ((long)(rows - 1) * a.ldA + ((krem + 7) & ~7)) * 2 : 0;
+    uintx4 rA, rB;
+    unsigned lds;
+    bool inA, inB;
+    auto load_begin = [&](unsigned stage) {
+        const __bf16 *qA = pA, *qB = pB;
+        if (a.combos > 1) {   // uniform
+            const bool second = combo >= a.parts6;
+            const int c = second ? combo - a.parts6 : combo;
+            if (second) {
+                qA += toA1;
+                qB += toB1;
+            }
+            if (a.parts6 == 6) {
+                qA += combo_part_a(c) * a.planeA;
+                qB += combo_part_b(c) * a.planeB;
+            }
         }
-        if constexpr (BT) {
-            pB += (long)kt * 64 * a.ldB + n0;
-            bytesB = krem > 0 ? ((long)(krem - 1) * a.ldB + ((a.N - n0 + 7) & ~7)) * 2 : 0;
-        } else {
-            const int span = GATED ? BN / 2 : BN, rows = a.N - n0 < span ? a.N - n0 : span;
-            pB += (long)n0 * a.ldB + kt * 64;
-            bytesB = krem > 0 ? ((long)(rows - 1) * a.ldB + ((krem + 7) & ~7)) * 2 : 0;
-        }
-        const uintx4 rA = make_rsrc(pA, bytesA), rB = make_rsrc(pB, bytesB);
-        const unsigned lds = __builtin_amdgcn_readfirstlane(lds0 + stage + wave * 1024);
-        const bool inA = AT || kchunkA < krem, inB = BT || kchunkB < krem;   // a straight row goes on into the next one
-#pragma unroll
-        for (int j = 0; j < LA; j++) load_to_lds(lds + j * NT * 16, inA ? offA[j] : 0x80000000u, rA);
-#pragma unroll
-        for (int j = 0; j < LB; j++) load_to_lds(lds + ABYTES + j * NT * 16, inB ? offB[j] : 0x80000000u, rB);
+        if (GATED && (wave & 2)) qB += toB1;
+        const int rows = krem < 32 ? krem : 32;
+        rA = make_rsrc(qA, !AT ? endA : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldA * 2) + endA : 0u);
+        rB = make_rsrc(qB, !BT ? endB : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldB * 2) + endB : 0u);
+        inA = AT || kchunkA < krem;   // a straight row goes on into the next one
+        inB = BT || kchunkB < krem;
+        lds = __builtin_amdgcn_readfirstlane(lds0 + stage + wave * 1024);
         if (++combo == a.combos) {
             combo = 0;
-            kt++;
+            krem -= 32;
+            pA += stepA;
+            pB += stepB;
         }
+    };
+    auto load_one = [&](int j) {
+        if (j < LA) load_to_lds(lds + j * NT * 16, inA ? offA[j < LA ? j : 0] : 0x80000000u, rA);
+        else load_to_lds(lds + ABYTES + (j - LA) * NT * 16, inB ? offB[j < LA ? 0 : j - LA] : 0x80000000u, rB);
     };
 
     // ---- where the fragments are read ----
     typedef __attribute__((address_space(3))) char lds_char;
-    unsigned rdA[AT ? 4 : 1], rdB[BT ? 4 : 1];
+    unsigned rdA[AT ? MF : 1], rdB[BT ? NF : 1];                 // (a T fragment's piece is permuted by the lane: an address each)
+    const int tk = q * 8 + (l16 >> 2), t16 = (l16 & 3) >> 1;     // T: the lane's k row and 16-byte half of a piece
+    const int chunk = (q ^ s_permutation(l16 >> 2)) * 16;
     if constexpr (AT) {
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-            rdA[x] = (q * 8 + (l16 >> 2)) * (BM * 2) + wm * (TM / 16) * 32 + ((x ^ (l16 >> 2)) * 32) + ((l16 & 3) >> 1) * 16 + (l16 & 1) * 8;
+        for (int x = 0; x < MF; x++) rdA[x] = tk * (BM * 2) + (((wm * MF + x) * 2 + t16) ^ t_permutation(tk)) * 16 + (l16 & 1) * 8;
     } else {
-        rdA[0] = (wm * TM + l16) * 128 + ((q ^ (l16 & 7)) * 16);
+        rdA[0] = (wm * TM + l16) * 64 + chunk;
     }
     if constexpr (BT) {
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-            rdB[x] = ABYTES + (q * 8 + (l16 >> 2)) * (BN * 2) + wn * (TN / 16) * 32 + ((x ^ (l16 >> 2)) * 32) + ((l16 & 3) >> 1) * 16 + (l16 & 1) * 8;
+        for (int x = 0; x < NF; x++) rdB[x] = ABYTES + tk * (BN * 2) + (((wn * NF + x) * 2 + t16) ^ t_permutation(tk)) * 16 + (l16 & 1) * 8;
     } else {
-        rdB[0] = ABYTES + (wn * TN + (l16 >> 2) * 16 + (l16 & 3)) * 128 + ((q ^ (l16 & 7)) * 16);
+        rdB[0] = ABYTES + (wn * TN + l16) * 64 + chunk;
     }
-    auto read_a = [&](unsigned stage, int ks, bf16x8 (&f)[MF]) {
-#pragma unroll
-        for (int i = 0; i < MF; i++) {
-            if constexpr (AT) {
-                const unsigned at = stage + rdA[i & 3] + (i >> 2) * 128 + ks * 32 * (BM * 2);
-                const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)((lds_char *)smem + at));
-                const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)((lds_char *)smem + at + 4 * (BM * 2)));
-                f[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            } else {
-                f[i] = *(const __attribute__((address_space(3))) bf16x8 *)((lds_char *)smem + stage + (rdA[0] ^ (ks * 64)) + i * 2048);
-            }
-        }
+    auto read_t = [&](unsigned at, int row_bytes) {   // k .. k+3 and k+4 .. k+7 of the lane's row
+        const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)((lds_char *)smem + at));
+        const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)((lds_char *)smem + at + 4 * row_bytes));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto read_b = [&](unsigned stage, int ks, bf16x8 (&f)[NF]) {
-#pragma unroll
-        for (int i = 0; i < NF; i++) {
-            if constexpr (BT) {
-                const unsigned at = stage + rdB[i & 3] + (i >> 2) * 128 + ks * 32 * (BN * 2);
-                const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)((lds_char *)smem + at));
-                const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)((lds_char *)smem + at + 4 * (BN * 2)));
-                f[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            } else {
-                f[i] = *(const __attribute__((address_space(3))) bf16x8 *)((lds_char *)smem + stage + (rdB[0] ^ (ks * 64)) + (i >> 2) * 8192 + (i & 3) * 512);
-            }
-        }
+    auto read_a = [&](unsigned stage, int i) -> bf16x8 {
+        if constexpr (AT) return read_t(stage + rdA[i], BM * 2);
+        else return *(const __attribute__((address_space(3))) bf16x8 *)((lds_char *)smem + stage + rdA[0] + i * 1024);
+    };
+    auto read_b = [&](unsigned stage, int i) -> bf16x8 {
+        if constexpr (BT) return read_t(stage + rdB[i], BN * 2);
+        else return *(const __attribute__((address_space(3))) bf16x8 *)((lds_char *)smem + stage + rdB[0] + i * 1024);
     };
 
     floatx4 acc[MF][NF];
@@ -285,97 +380,127 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     for (int i = 0; i < MF; i++)
 #pragma unroll
         for (int j = 0; j < NF; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const bf16x8 (&fa)[MF], const bf16x8 (&fb)[NF]) {
+    // The MFMAs of a step, row by row, with the loads of the step four ahead and the reads of the next one spread between
+    // the rows, so that none waits behind a queue of the other.
+    auto step = [&](const bf16x8 (&fa)[MF], const bf16x8 (&fb)[NF], bf16x8 (&na)[MF], bf16x8 (&nb)[NF], unsigned next) {
+        constexpr int READS = MF + NF, LOADS = LA + LB;
 #pragma unroll
-        for (int i = 0; i < MF; i++)
+        for (int i = 0; i < MF; i++) {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++)
+                if (j * MF / LOADS == i) load_one(j);
+            // B's fragments first: the next step's first row needs all of them
+#pragma unroll
+            for (int r = 0; r < READS; r++)
+                if (r * MF / READS == i) {
+                    if (r < NF) nb[r] = read_b(next, r);
+                    else na[r - NF] = read_a(next, r - NF);
+                }
 #pragma unroll
             for (int j = 0; j < NF; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     bf16x8 a0[MF], b0[NF], a1[MF], b1[NF];
-    load_step(0);
-    load_step(STAGE);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LA + LB) : "memory");
-    read_a(0, 0, a0);
-    read_b(0, 0, b0);
-    unsigned stage = 0;
-    for (int t = 0; t < left; t++) {
-        read_a(stage, 1, a1);
-        read_b(stage, 1, b1);
-        multiply(a0, b0);
-        // all reads of this step's tiles are done and the next step's tiles have landed, for every wavefront
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        load_step(stage);
-        stage ^= STAGE;
-        read_a(stage, 0, a0);
-        read_b(stage, 0, b0);
-        multiply(a1, b1);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        load_begin(r * STAGE);
+#pragma unroll
+        for (int j = 0; j < LA + LB; j++) load_one(j);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load may reach LDS after the workgroup has gone
-
-    // ---- out ----
-    // Column of fragment group g (64 columns), run j; gated: of the gate's fragment g + j and its partner g + j + 2.
-    auto column = [&](int g, int j) {
-        const int col = wn * TN + g * 16;
-        return n0 + (GATED ? col / 2 + q * 8 + j * 4 : col + (PERM ? q * 16 + j * 4 : j * 16 + q * 4));
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * (LA + LB)) : "memory");
+#pragma unroll
+    for (int i = 0; i < NF; i++) b0[i] = read_b(0, i);
+#pragma unroll
+    for (int i = 0; i < MF; i++) a0[i] = read_a(0, i);
+    unsigned stage = 0;
+    // A step begins when this step's fragments are in every wavefront's registers (its buffer is free) and the next step's
+    // tiles have landed, two more steps' loads being on their way.
+    auto next_stage = [&]() {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LA + LB)) : "memory");
+        load_begin(stage);
+        stage = stage + STAGE == RING ? 0 : stage + STAGE;
+        __builtin_amdgcn_sched_barrier(0);
     };
-    constexpr int RUNS = GATED ? 2 : 4;
+    for (int t = 0; t < left; t += 2) {   // (an odd number of steps ends with one of zeros: the loads beyond the last are none)
+        next_stage();
+        step(a0, b0, a1, b1, stage);
+        next_stage();
+        step(a1, b1, a0, b0, stage);
+    }
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // every load into LDS has landed, every read of it is done
+
+    // ---- out: two fragment rows (32 rows of C) at a time through the wavefront's part of LDS ----
+    static_assert(TN == 64, "a wavefront's rows are 64 columns");
+    constexpr int ROW = 68;                              // floats from row to row: 16 bytes past a multiple of the banks
+    constexpr int LANES = GATED ? 4 : 8;                 // lanes of a row, eight columns each (gated: eight of each filter)
+    constexpr int AT_ONCE = 64 / LANES;
+    static_assert(WM * WN * 32 * ROW * 4 <= (int)RING, "the ring holds the parts");
+    float *const part = reinterpret_cast<float *>(smem) + wave * (32 * ROW);
+    const int at = (lane % LANES) * 8, n = n0 + wn * (GATED ? 32 : 64) + at;
     unsigned again = 0;   // fp32: runs with a NaN among them, computed once more below
 #pragma unroll
-    for (int i = 0; i < MF; i++) {
-        const int m = m0 + wm * TM + i * 16 + l16;
-        if (m >= a.M) continue;
+    for (int i = 0; i < MF; i += 2) {
 #pragma unroll
-        for (int g = 0; g < NF; g += 4) {
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int j = 0; j < RUNS; j++) {
-                const int n = column(g, j);
-                if (n >= a.N) continue;
-                const floatx4 v = acc[i][g + j], u = acc[i][GATED ? g + j + 2 : g + j];
-                if constexpr (OUT == DENSE_PARTIAL || OUT == DENSE_PARTIAL_GATED) {
-                    float *dst = a.partial + ((long)piece * a.M + m) * a.columns + n;
-                    if ((a.N & 3) == 0) {
-                        *reinterpret_cast<floatx4 *>(dst) = v;
-                        if constexpr (GATED) *reinterpret_cast<floatx4 *>(dst + a.N) = u;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (n + e < a.N) {
-                                dst[e] = v[e];
-                                if constexpr (GATED) dst[a.N + e] = u[e];
-                            }
-                    }
+            for (int j = 0; j < NF; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[i + h][j];
+        wave_fence();
+#pragma unroll 1
+        for (int y = 0; y < 32; y += AT_ONCE) {
+            const int row = y + lane / LANES;
+            const long m = m0 + wm * TM + i * 16 + row;
+            float v[8], u[8];
+            run_load(part + row * ROW + at, v);
+            if constexpr (GATED) run_load(part + row * ROW + 32 + at, u);
+            if (m >= a.M || n >= a.N) continue;
+            if constexpr (OUT == DENSE_PARTIAL || OUT == DENSE_PARTIAL_GATED) {
+                float *dst = a.partial + (piece * (long)a.M + m) * a.columns + n;
+                if ((a.N & 3) == 0 && n + 8 <= a.N) {
+                    run_store(dst, v);
+                    if constexpr (GATED) run_store(dst + a.N, u);
                 } else {
-                    if constexpr (__is_same(T, float)) {
-                        const float sum = (v[0] + v[1]) + (v[2] + v[3]) + (GATED ? (u[0] + u[1]) + (u[2] + u[3]) : 0.f);
-                        if (sum != sum) {   // (also where infinities of both signs meet: no harm)
-                            again |= 1u << (i * (NF / 4 * RUNS) + g / 4 * RUNS + j);
-                            continue;
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (n + e < a.N) {
+                            dst[e] = v[e];
+                            if constexpr (GATED) dst[a.N + e] = u[e];
                         }
-                    }
-                    if constexpr (GATED) dense_finish4_gated<T>(a.ep, v, u, m, n, a.N);
-                    else dense_finish4<T>(a.ep, v, m, n, a.N);
                 }
+            } else {
+                if constexpr (__is_same(T, float)) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
+                    if (sum != sum) {   // (also where infinities of both signs meet: no harm)
+                        again |= 1u << (i / 2 * (32 / AT_ONCE) + y / AT_ONCE);
+                        continue;
+                    }
+                }
+                if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n, a.N);
+                else dense_finish<T>(a.ep, v, m, n, a.N);
             }
         }
+        wave_fence();
     }
     if constexpr (__is_same(T, float) && (OUT == DENSE_PLAIN || OUT == DENSE_GATED)) {
-        static_assert(MF * (NF / 4) * RUNS <= 32, "one bit per run");
+        static_assert(MF / 2 * (32 / AT_ONCE) <= 32, "one bit per run");
         while (again) {
-            const int bit = __ffs(again) - 1, i = bit / (NF / 4 * RUNS), g = bit / RUNS % (NF / 4) * 4, j = bit % RUNS;
+            const int bit = __ffs(again) - 1;
             again &= again - 1;
-            const long m = m0 + wm * TM + i * 16 + l16;
-            const int n = column(g, j);
-            floatx4 v{0.f, 0.f, 0.f, 0.f}, u = v;
-            for (int e = 0; e < 4 && n + e < a.N; e++) {
-                const float x = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.planeA, a.B[0], a.B[1],
-                                              BT ? n + e : (n + e) * a.ldB, BT ? a.ldB : 1, a.planeB, GATED ? 1 : a.combos / a.parts6, a.K);
-                const float y = GATED ? dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.planeA, a.B[1], a.B[1], (n + e) * a.ldB, 1, a.planeB, 1, a.K) : 0.f;
-                v[0] = e == 0 ? x : v[0], v[1] = e == 1 ? x : v[1], v[2] = e == 2 ? x : v[2], v[3] = e == 3 ? x : v[3];
-                u[0] = e == 0 ? y : u[0], u[1] = e == 1 ? y : u[1], u[2] = e == 2 ? y : u[2], u[3] = e == 3 ? y : u[3];
+            const long m = m0 + wm * TM + bit * AT_ONCE + lane / LANES;
+            for (int e = 0; e < 8 && n + e < a.N; e++) {
+                float v[1], u[1] = {0.f};
+                v[0] = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.planeA, a.B[0], a.B[1], BT ? n + e : (n + e) * a.ldB,
+                                     BT ? a.ldB : 1, a.planeB, GATED ? 1 : a.combos / a.parts6, a.K);
+                if constexpr (GATED) {
+                    u[0] = dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.planeA, a.B[1], a.B[1], (n + e) * a.ldB, 1, a.planeB, 1, a.K);
+                    dense_finish_gated<T>(a.ep, v, u, m, n + e, a.N);
+                } else {
+                    dense_finish<T>(a.ep, v, m, n + e, a.N);
+                }
             }
-            if constexpr (GATED) dense_finish4_gated<T>(a.ep, v, u, m, n, a.N);
-            else dense_finish4<T>(a.ep, v, m, n, a.N);
         }
     }
 }

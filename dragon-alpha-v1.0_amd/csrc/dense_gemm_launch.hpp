@@ -12,7 +12,7 @@ hipError_t launch_dense_tile_tt(hipStream_t s, const DenseTileArgs &a, bool big,
 template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN>
 inline hipError_t launch_dense_tile(hipStream_t s, const DenseTileArgs &a)
 {
-    constexpr size_t lds = 2 * (BM + BN) * 128;
+    constexpr size_t lds = 4 * (BM + BN) * 64;
     const hipError_t e = ensure_dynamic_lds<dense_tile_kernel<T, AT, BT, OUT, BM, BN, WM, WN>>(lds);
     if (e != hipSuccess) return e;
     const unsigned blocks = (unsigned)a.tiles_m * (unsigned)a.tiles_n * (unsigned)a.split;
