@@ -149,6 +149,7 @@ int quads_aligned(int type, std::initializer_list<const void *> p, std::initiali
     return 1;
 }
 
+
 // ---- workspaces: the same sequence of blocks for the query (base NULL) and the call --------------------------------
 struct ForwardRoom {
     void *X, *W[2];
@@ -159,6 +160,7 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
 {
     Scratch ws(base);
     ForwardRoom r{};
+    if (dense_few_rows_preferred(type == ALPHA_DENSE_F32, gated, N, OC, IC)) return r;   // operands as they are, no pieces
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC));
     r.partial_bytes = dense_product_partial_bytes(N, OC, IC, parts_of(type), 1, gated);
@@ -196,6 +198,22 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
 int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, int64_t ldX, const void *W, int64_t ldW, const void *W2, int64_t ldW2,
             const DenseEpilogue &ep, int N, int IC, int OC, void *workspace)
 {
+    if (dense_few_rows_preferred(type == ALPHA_DENSE_F32, gated, N, OC, IC)) {
+        DenseFewRows a{};
+        a.X = X;
+        a.ldX = ldX;
+        a.W = W;
+        a.ldW = ldW;
+        a.W2 = W2;
+        a.ldW2 = ldW2;
+        a.f32 = type == ALPHA_DENSE_F32;
+        a.gated = gated;
+        a.M = N;
+        a.N = OC;
+        a.K = IC;
+        a.ep = ep;
+        return hip_status(launch_dense_few_rows(s, a), fn);
+    }
     const ForwardRoom room = forward_room(type, N, IC, OC, gated, workspace);
     DenseProduct p{};
     p.parts = parts_of(type);

@@ -114,6 +114,7 @@ struct DenseProduct {
     size_t partial_bytes;
 };
 size_t dense_product_partial_bytes(int M, int N, int K, int parts, int sources, int gated);
+double dense_product_us(int M, int N, int K, int parts, int sources, int gated);   // the plan's estimate
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p);
 
 // Few rows, operands as they are (dense_few_rows.hip).
@@ -124,6 +125,9 @@ struct DenseFewRows {
     int M, N, K;
     DenseEpilogue ep;
 };
+
+bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K);
+hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);
 
 // dst planes <- src[rows, cols]: fp32 in three parts, bf16 as it is; row stride ld (multiple of 8), columns cols .. ld zero.
 hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, __bf16 *dst, long ld, long plane);

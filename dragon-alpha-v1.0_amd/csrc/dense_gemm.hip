@@ -15,6 +15,7 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
         const int n = (int)(i - m * quads) * 4;
         floatx4 v{0.f, 0.f, 0.f, 0.f}, u = v;
         const float *src = a.partial + (long)m * a.columns + n;
+#pragma unroll 4
         for (int p = 0; p < a.split; p++, src += (long)a.M * a.columns) {
             if ((a.columns & 3) == 0 && (a.N & 3) == 0) {
                 v += *reinterpret_cast<const floatx4 *>(src);
@@ -48,35 +49,39 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
 namespace {
 
 struct Plan {
-    bool big;
+    DenseTile tile;
     int split, per, tiles_m, tiles_n, steps;
+    double us;
 };
 
-// Tile shape and cut: the least of a simple estimate of the device's time. `room`: bytes for the pieces.
+// Tile shape and cut of the reduction: the least of an estimate of the device's time, its constants measured on NT products
+// of 256 x 256 x 256 to 8192 x 4096 x 4096 (a workgroup's step with the device nearly empty and full, 256 / 256 x 128 / 128:
+// 0.57 / 0.34 / 0.36 and 0.72 / 0.48 / 0.59 us, the last with two workgroups on a compute unit). `room`: bytes for the pieces.
 Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t room)
 {
+    static constexpr double empty[DENSE_TILES] = {0.57, 0.34, 0.36}, full[DENSE_TILES] = {0.72, 0.48, 0.59}, fixed[DENSE_TILES] = {6.5, 5.0, 3.0};
     const int cus = std::max(1, device_cu_count());
-    const int nk = std::max(1, (K + 31) / 32), steps = nk * (parts == 3 ? 6 : 1) * sources;
-    const double out_bytes = (double)M * N * (gated ? 2 : 1) * 4;
+    const int nk = std::max(1, (K + 31) / 32), combos = (parts == 3 ? 6 : 1) * sources, steps = nk * combos;
+    const double outputs = (double)M * N * (gated ? 2 : 1), bytes_per_us = 4.2e6;
     Plan best{};
-    double best_us = 1e30;
-    for (int big = 0; big < 2; big++) {
-        const int bm = big ? 256 : 128, bn = (big ? 256 : 128) / (gated ? 2 : 1);
-        const int tm = (M + bm - 1) / bm, tn = (N + bn - 1) / bn;
-        const long tiles = (long)tm * tn, slots = (long)cus * (big ? 1 : 2);
+    best.us = 1e30;
+    for (int tile = 0; tile < DENSE_TILES; tile++) {
+        const int bm = DENSE_TILE_M[tile], bn = DENSE_TILE_N[tile] / (gated ? 2 : 1);
+        const int tm = (int)(((long)M + bm - 1) / bm), tn = (N + bn - 1) / bn;
+        const long tiles = (long)tm * tn;
         for (int split = 1; split <= 64; split++) {
             // whole k steps: a piece holds all parts of its products, so none leaves fp32's range that the sum would not
             // (and an even number of steps: the kernel's loop does two at a time)
-            const int combos = steps / nk, per = (nk + 2 * split - 1) / (2 * split) * 2 * combos;
-            if (split > 1 && (per < 8 || (long)split * M * N * (gated ? 2 : 1) * 4 > (long)room)) break;
+            const int per = (nk + 2 * split - 1) / (2 * split) * 2 * combos;
+            if (split > 1 && (per < 8 || split * outputs * 4 > (double)room)) break;
             if ((steps + per - 1) / per != split) continue;   // every piece has a step
-            const long rounds = (tiles * split + slots - 1) / slots;
-            double us = rounds * (per * (big ? 0.65 : 0.4) + 3.0);
-            if (split > 1) us += 3.0 + out_bytes * (split * 2 + 1) / 4e6;
-            if (us < best_us) {
-                best_us = us;
-                best = Plan{big != 0, split, per, tm, tn, steps};
-            }
+            const long groups = tiles * split;
+            const bool pairs = tile == DENSE_TILE_128 && groups > cus;
+            const long slots = pairs ? 2l * cus : cus, rounds = (groups + slots - 1) / slots;
+            const double fill = std::min(1.0, (double)groups / slots);
+            double us = 3.5 + rounds * (per * (tile == DENSE_TILE_128 ? (pairs ? full[tile] : empty[tile]) : empty[tile] + (full[tile] - empty[tile]) * fill) + fixed[tile]);
+            us += split > 1 ? 5.0 + outputs * (8.0 * split + 2) / bytes_per_us : outputs * (parts == 3 ? 4 : 2) / bytes_per_us;
+            if (us < best.us) best = Plan{(DenseTile)tile, split, per, tm, tn, steps, us};
         }
     }
     return best;
@@ -90,6 +95,8 @@ size_t dense_product_partial_bytes(int M, int N, int K, int parts, int sources, 
     const Plan p = make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60);
     return p.split > 1 ? (size_t)p.split * M * N * (gated ? 2 : 1) * 4 : 0;
 }
+
+double dense_product_us(int M, int N, int K, int parts, int sources, int gated) { return make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60).us; }
 
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
 {
@@ -118,10 +125,10 @@ hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
     a.partial = p.partial;
     a.columns = p.gated ? 2 * p.N : p.N;
     hipError_t e;
-    if (p.a_t) e = launch_dense_tile_tt(s, a, plan.big, p.f32);
-    else if (p.b_t) e = launch_dense_tile_st(s, a, plan.big, p.f32);
-    else if (p.gated) e = launch_dense_tile_gated(s, a, plan.big, p.f32);
-    else e = launch_dense_tile_ss(s, a, plan.big, p.f32);
+    if (p.a_t) e = launch_dense_tile_tt(s, a, plan.tile, p.f32);
+    else if (p.b_t) e = launch_dense_tile_st(s, a, plan.tile, p.f32);
+    else if (p.gated) e = launch_dense_tile_gated(s, a, plan.tile, p.f32);
+    else e = launch_dense_tile_ss(s, a, plan.tile, p.f32);
     if (e != hipSuccess || a.split == 1) return e;
     const long quads = (p.N + 3) / 4, work = quads * p.M;
     const FastDiv d = make_fastdiv((uint32_t)quads);

@@ -1,7 +1,7 @@
 // The dense product's tile kernel: C[m, n] = sum_k A(m, k) B(n, k), bf16 operands, fp32 sums, on v_mfma_f32_16x16x32_bf16.
 //
 // A workgroup computes BM x BN of C in steps of 32 k. A step's tiles go from memory straight into LDS (128-bit buffer
-// loads with LDS as their target) through a ring of four buffers, four steps ahead; a wavefront owns BM/WM x BN/WN of C in
+// loads with LDS as their target) through a ring of STAGES buffers, that many steps ahead; a wavefront owns BM/WM x BN/WN of C in
 // registers and reads the operand fragments of a step while it multiplies those of the step before, so the one barrier of
 // a step falls between two runs of MFMAs whose operands are in registers already.
 // Operands may be stored with k along their rows (row r: k = 0, 1, ..: "straight") or with k as the rows ("T"). Straight
@@ -15,7 +15,9 @@
 // bytes: stored from the registers as they are, 4096 x 4096 of bf16 took 17 us to write, this way 10.
 // Gated: of every 64 tile columns 32 are of one filter and 32, the same ones, of the other.
 #pragma once
-#include "dense_common.hpp"
+#include "dense_finish.hpp"
+
+#include <type_traits>
 
 namespace alpha {
 
@@ -75,144 +77,13 @@ static __device__ __attribute__((noinline)) float dense_element(const __bf16 *A0
     return acc;
 }
 
-// R consecutive elements of a row, aligned to groups of four.
-template <int R, typename T>
-static __device__ __forceinline__ void run_load(const T *p, float (&v)[R])
+// f(0), f(1), .. f(N - 1) with constants: unrolled whatever its size
+template <int N, int I = 0, typename F>
+static __device__ __forceinline__ void for_each(F &&f)
 {
-#pragma unroll
-    for (int i = 0; i < R; i += 4) {
-        const floatx4 q = quad_load(p + i);
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[i + e] = q[e];
-    }
-}
-template <int R, typename T>
-static __device__ __forceinline__ void run_store(T *p, const float (&v)[R])
-{
-    if constexpr (R == 8 && sizeof(T) == 2) {   // one 128-bit store (the hardware takes 8-byte alignment)
-        bf16x8 q;
-#pragma unroll
-        for (int e = 0; e < 8; e++) q[e] = (T)v[e];
-        __builtin_memcpy(__builtin_assume_aligned(p, 8), &q, 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < R; i += 4) quad_store(p + i, floatx4{v[i], v[i + 1], v[i + 2], v[i + 3]});
-    }
-}
-template <int R>
-static __device__ __forceinline__ void run_act(int act, float (&v)[R], float k)
-{
-    switch (act) {   // one branch for the run
-    case ALPHA_DENSE_ACT_LEAKY_RELU:
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_LEAKY_RELU, v[e], k);
-        break;
-    case ALPHA_DENSE_ACT_GELU:
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_GELU, v[e], k);
-        break;
-    case ALPHA_DENSE_ACT_SILU:
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_SILU, v[e], k);
-        break;
-    case ALPHA_DENSE_ACT_SIGMOID:
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_SIGMOID, v[e], k);
-        break;
-    default: break;
-    }
-}
-
-// The epilogues of R consecutive columns n .. n+R-1 of row m (fewer at the right edge).
-template <typename T, int R>
-static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n, int N)
-{
-    const bool second = ep.row2 > 0 && m >= ep.row2;
-    if (ep.row2 > 0 && !second && m >= ep.rows1) return;   // a row between two stacked products
-    T *Y = static_cast<T *>(second ? ep.Y2 : ep.Y) + (second ? (m - ep.row2) * ep.ldY2 : m * ep.ldY) + n;
-    const T *bias = static_cast<const T *>(ep.bias), *res = static_cast<const T *>(ep.R);
-    T *Z = static_cast<T *>(ep.Z);
-    const bool whole = R % 4 == 0 && ep.vec && n + R <= N;
-    float t[R];
-    if (bias) {
-        if constexpr (R % 4 == 0)
-            if (whole) run_load(bias + n, t);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(bias + n + e) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] += t[e];
-    }
-    if (Z) {
-        if constexpr (R % 4 == 0)
-            if (whole) run_store(Z + m * ep.ldZ + n, v);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < R; e++)
-                if (n + e < N) dense_store(Z + m * ep.ldZ + n + e, v[e]);
-        }
-    }
-    run_act(ep.act, v, ep.slope);
-    if (res) {
-        if constexpr (R % 4 == 0)
-            if (whole) run_load(res + m * ep.ldR + n, t);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(res + m * ep.ldR + n + e) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] += t[e];
-    }
-    if constexpr (R % 4 == 0)
-        if (whole) run_store(Y, v);
-    if (!whole) {
-#pragma unroll
-        for (int e = 0; e < R; e++)
-            if (n + e < N) dense_store(Y + e, v[e]);
-    }
-}
-
-template <typename T, int R>
-static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &ep, float (&g)[R], float (&u)[R], long m, int n, int N)
-{
-    T *Y = static_cast<T *>(ep.Y) + m * ep.ldY + n;
-    const bool whole = R % 4 == 0 && ep.vec && n + R <= N;
-#pragma unroll
-    for (int which = 0; which < 2; which++) {
-        float(&v)[R] = which ? u : g;
-        const T *bias = static_cast<const T *>(which ? ep.bias2 : ep.bias);
-        T *Z = static_cast<T *>(which ? ep.Z2 : ep.Z) + m * (which ? ep.ldZ2 : ep.ldZ) + n;
-        if (bias) {
-            float t[R];
-            if constexpr (R % 4 == 0)
-                if (whole) run_load(bias + n, t);
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(bias + n + e) : 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < R; e++) v[e] += t[e];
-        }
-        if (which ? ep.Z2 != nullptr : ep.Z != nullptr) {
-            if constexpr (R % 4 == 0)
-                if (whole) run_store(Z, v);
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < R; e++)
-                    if (n + e < N) dense_store(Z + e, v[e]);
-            }
-        }
-    }
-    run_act(ep.act, g, ep.slope);
-#pragma unroll
-    for (int e = 0; e < R; e++) g[e] *= u[e];
-    if constexpr (R % 4 == 0)
-        if (whole) run_store(Y, g);
-    if (!whole) {
-#pragma unroll
-        for (int e = 0; e < R; e++)
-            if (n + e < N) dense_store(Y + e, g[e]);
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        for_each<N, I + 1>(f);
     }
 }
 
@@ -232,12 +103,12 @@ static __device__ __forceinline__ int t_permutation(int k) { return ((k & 3) | (
 // four groups of rows must come to four different chunks: 0, 3, 2, 1 for g = 0 .. 3. Counted: no conflicts.
 static __device__ __forceinline__ int s_permutation(int g) { return (g & 1) | ((g ^ (g >> 1)) & 1) << 1; }
 
-template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN>
+template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const DenseTileArgs a)
 {
     constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
     constexpr int LA = BM * 4 / NT, LB = BN * 4 / NT;       // 16-byte loads of a thread per step
-    constexpr unsigned ABYTES = BM * 64, BBYTES = BN * 64, STAGE = ABYTES + BBYTES, RING = 4 * STAGE;
+    constexpr unsigned ABYTES = BM * 64, BBYTES = BN * 64, STAGE = ABYTES + BBYTES, RING = STAGES * STAGE;
     constexpr bool GATED = OUT == DENSE_GATED || OUT == DENSE_PARTIAL_GATED;
     static_assert(TM % 16 == 0 && TN % 64 == 0 && LA >= 1 && LB >= 1 && NT % 256 == 0, "tile shape");
     extern __shared__ char smem[];
@@ -311,32 +182,41 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     uintx4 rA, rB;
     unsigned lds;
     bool inA, inB;
-    auto load_begin = [&](unsigned stage) {
-        const __bf16 *qA = pA, *qB = pB;
-        if (a.combos > 1) {   // uniform
-            const bool second = combo >= a.parts6;
-            const int c = second ? combo - a.parts6 : combo;
-            if (second) {
-                qA += toA1;
-                qB += toB1;
+    const __bf16 *qA, *qB;
+    // the descriptors of the next step's loads, in four parts that the main loop spreads between its MFMAs
+    auto load_begin = [&](unsigned stage, int part) {
+        if (part == 0) {
+            qA = pA;
+            qB = pB;
+            if (a.combos > 1) {   // uniform
+                const bool second = combo >= a.parts6;
+                const int c = second ? combo - a.parts6 : combo;
+                if (second) {
+                    qA += toA1;
+                    qB += toB1;
+                }
+                if (a.parts6 == 6) {
+                    qA += combo_part_a(c) * a.planeA;
+                    qB += combo_part_b(c) * a.planeB;
+                }
             }
-            if (a.parts6 == 6) {
-                qA += combo_part_a(c) * a.planeA;
-                qB += combo_part_b(c) * a.planeB;
+            if (GATED && (wave & 2)) qB += toB1;
+        } else if (part == 1) {
+            const int rows = krem < 32 ? krem : 32;
+            rA = make_rsrc(qA, !AT ? endA : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldA * 2) + endA : 0u);
+            inA = AT || kchunkA < krem;   // a straight row goes on into the next one
+        } else if (part == 2) {
+            const int rows = krem < 32 ? krem : 32;
+            rB = make_rsrc(qB, !BT ? endB : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldB * 2) + endB : 0u);
+            inB = BT || kchunkB < krem;
+        } else {
+            lds = __builtin_amdgcn_readfirstlane(lds0 + stage + wave * 1024);
+            if (++combo == a.combos) {
+                combo = 0;
+                krem -= 32;
+                pA += stepA;
+                pB += stepB;
             }
-        }
-        if (GATED && (wave & 2)) qB += toB1;
-        const int rows = krem < 32 ? krem : 32;
-        rA = make_rsrc(qA, !AT ? endA : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldA * 2) + endA : 0u);
-        rB = make_rsrc(qB, !BT ? endB : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldB * 2) + endB : 0u);
-        inA = AT || kchunkA < krem;   // a straight row goes on into the next one
-        inB = BT || kchunkB < krem;
-        lds = __builtin_amdgcn_readfirstlane(lds0 + stage + wave * 1024);
-        if (++combo == a.combos) {
-            combo = 0;
-            krem -= 32;
-            pA += stepA;
-            pB += stepB;
         }
     };
     auto load_one = [&](int j) {
@@ -380,62 +260,63 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     for (int i = 0; i < MF; i++)
 #pragma unroll
         for (int j = 0; j < NF; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    // The MFMAs of a step, row by row, with the loads of the step four ahead and the reads of the next one spread between
-    // the rows, so that none waits behind a queue of the other.
-    auto step = [&](const bf16x8 (&fa)[MF], const bf16x8 (&fb)[NF], bf16x8 (&na)[MF], bf16x8 (&nb)[NF], unsigned next) {
-        constexpr int READS = MF + NF, LOADS = LA + LB;
-#pragma unroll
-        for (int i = 0; i < MF; i++) {
-#pragma unroll
-            for (int j = 0; j < LOADS; j++)
-                if (j * MF / LOADS == i) load_one(j);
-            // B's fragments first: the next step's first row needs all of them
-#pragma unroll
-            for (int r = 0; r < READS; r++)
-                if (r * MF / READS == i) {
-                    if (r < NF) nb[r] = read_b(next, r);
+    // The MFMAs of a step. Between them, one at a time, so that none keeps the next MFMA waiting: the reads of the next
+    // step's fragments (B's first, since its first row needs all of them), the loads of the step STAGES ahead (into the
+    // buffer of this step's tiles, which are in registers), and towards the end the scalar arithmetic of the next loads. So
+    // nothing stands between the barrier and the MFMAs, and the wait before the next barrier finds the reads done.
+    unsigned stage = 0;
+    auto step = [&](const bf16x8 (&fa)[MF], const bf16x8 (&fb)[NF], bf16x8 (&na)[MF], bf16x8 (&nb)[NF]) {
+        constexpr int READS = MF + NF, LOADS = LA + LB, ALL = MF * NF, EARLY = ALL * 3 / 4;
+        // this step's fragments are in every wavefront's registers and the next step's tiles have landed, STAGES - 2 more on their way
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * LOADS) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned next = stage + STAGE == RING ? 0 : stage + STAGE;
+        for_each<ALL>([&](auto at) __attribute__((always_inline)) {
+            constexpr int x = at;
+            for_each<READS>([&](auto read) __attribute__((always_inline)) {
+                constexpr int r = read;
+                if constexpr (r * EARLY / READS == x) {
+                    if constexpr (r < NF) nb[r] = read_b(next, r);
                     else na[r - NF] = read_a(next, r - NF);
                 }
-#pragma unroll
-            for (int j = 0; j < NF; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+            });
+            for_each<LOADS>([&](auto load) __attribute__((always_inline)) {
+                constexpr int j = load;
+                if constexpr ((2 * j + 1) * EARLY / (2 * LOADS) == x) load_one(j);
+            });
+            for_each<4>([&](auto c) __attribute__((always_inline)) {
+                if constexpr (EARLY + c * (ALL - EARLY) / 4 == x) load_begin(next, c);
+            });
+            acc[x / NF][x % NF] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[x % NF], fa[x / NF], acc[x / NF][x % NF], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
+        stage = next;
     };
 
     bf16x8 a0[MF], b0[NF], a1[MF], b1[NF];
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        load_begin(r * STAGE);
+    for (int r = 0; r < STAGES; r++) {
+        for (int c = 0; c < 4; c++) load_begin(r * STAGE, c);
 #pragma unroll
         for (int j = 0; j < LA + LB; j++) load_one(j);
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * (LA + LB)) : "memory");
+    for (int c = 0; c < 4; c++) load_begin(0, c);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * (LA + LB)) : "memory");
 #pragma unroll
     for (int i = 0; i < NF; i++) b0[i] = read_b(0, i);
 #pragma unroll
     for (int i = 0; i < MF; i++) a0[i] = read_a(0, i);
-    unsigned stage = 0;
-    // A step begins when this step's fragments are in every wavefront's registers (its buffer is free) and the next step's
-    // tiles have landed, two more steps' loads being on their way.
-    auto next_stage = [&]() {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LA + LB)) : "memory");
-        load_begin(stage);
-        stage = stage + STAGE == RING ? 0 : stage + STAGE;
-        __builtin_amdgcn_sched_barrier(0);
-    };
     for (int t = 0; t < left; t += 2) {   // (an odd number of steps ends with one of zeros: the loads beyond the last are none)
-        next_stage();
-        step(a0, b0, a1, b1, stage);
-        next_stage();
-        step(a1, b1, a0, b0, stage);
+        step(a0, b0, a1, b1);
+        step(a1, b1, a0, b0);
     }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // every load into LDS has landed, every read of it is done
 
     // ---- out: two fragment rows (32 rows of C) at a time through the wavefront's part of LDS ----
-    static_assert(TN == 64, "a wavefront's rows are 64 columns");
     constexpr int ROW = 68;                              // floats from row to row: 16 bytes past a multiple of the banks
     constexpr int LANES = GATED ? 4 : 8;                 // lanes of a row, eight columns each (gated: eight of each filter)
-    constexpr int AT_ONCE = 64 / LANES;
+    constexpr int AT_ONCE = 64 / LANES, TURNS = 32 / AT_ONCE;
+    static_assert(TN == 64, "a wavefront's rows are 64 columns");
     static_assert(WM * WN * 32 * ROW * 4 <= (int)RING, "the ring holds the parts");
     float *const part = reinterpret_cast<float *>(smem) + wave * (32 * ROW);
     const int at = (lane % LANES) * 8, n = n0 + wn * (GATED ? 32 : 64) + at;
@@ -445,7 +326,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int j = 0; j < NF; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[i + h][j];
+            for (int j = 0; j < 4; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[i + h][j];
         wave_fence();
 #pragma unroll 1
         for (int y = 0; y < 32; y += AT_ONCE) {
@@ -474,7 +355,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
 #pragma unroll
                     for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
                     if (sum != sum) {   // (also where infinities of both signs meet: no harm)
-                        again |= 1u << (i / 2 * (32 / AT_ONCE) + y / AT_ONCE);
+                        again |= 1u << (i / 2 * TURNS + y / AT_ONCE);
                         continue;
                     }
                 }
@@ -485,11 +366,11 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
         wave_fence();
     }
     if constexpr (__is_same(T, float) && (OUT == DENSE_PLAIN || OUT == DENSE_GATED)) {
-        static_assert(MF / 2 * (32 / AT_ONCE) <= 32, "one bit per run");
+        static_assert(MF / 2 * TURNS <= 32, "one bit per run");
         while (again) {
             const int bit = __ffs(again) - 1;
             again &= again - 1;
-            const long m = m0 + wm * TM + bit * AT_ONCE + lane / LANES;
+            const long m = m0 + wm * TM + bit / TURNS * 32 + bit % TURNS * AT_ONCE + lane / LANES;
             for (int e = 0; e < 8 && n + e < a.N; e++) {
                 float v[1], u[1] = {0.f};
                 v[0] = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.planeA, a.B[0], a.B[1], BT ? n + e : (n + e) * a.ldB,

@@ -4,32 +4,43 @@
 
 namespace alpha {
 
-hipError_t launch_dense_tile_ss(hipStream_t s, const DenseTileArgs &a, bool big, int f32);      // both straight
-hipError_t launch_dense_tile_gated(hipStream_t s, const DenseTileArgs &a, bool big, int f32);
-hipError_t launch_dense_tile_st(hipStream_t s, const DenseTileArgs &a, bool big, int f32);      // B with k as its rows
-hipError_t launch_dense_tile_tt(hipStream_t s, const DenseTileArgs &a, bool big, int f32);      // both with k as their rows
+// The tile shapes: 256 x 256 (eight wavefronts, two by four), 256 x 128 (four by two), 128 x 128 (four wavefronts), each a
+// ring of four buffers: 128, 96 and 64 KB of LDS, so two workgroups of the last share a compute unit.
+enum DenseTile { DENSE_TILE_256, DENSE_TILE_256_128, DENSE_TILE_128, DENSE_TILES };
+constexpr int DENSE_TILE_M[DENSE_TILES] = {256, 256, 128}, DENSE_TILE_N[DENSE_TILES] = {256, 128, 128};
+
+hipError_t launch_dense_tile_ss(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32);      // both straight
+hipError_t launch_dense_tile_gated(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32);
+hipError_t launch_dense_tile_st(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32);      // B with k as its rows
+hipError_t launch_dense_tile_tt(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32);      // both with k as their rows
 
 template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN>
 inline hipError_t launch_dense_tile(hipStream_t s, const DenseTileArgs &a)
 {
-    constexpr size_t lds = 4 * (BM + BN) * 64;
-    const hipError_t e = ensure_dynamic_lds<dense_tile_kernel<T, AT, BT, OUT, BM, BN, WM, WN>>(lds);
+    constexpr int stages = 4;
+    constexpr size_t lds = stages * (BM + BN) * 64;
+    constexpr auto kernel = dense_tile_kernel<T, AT, BT, OUT, BM, BN, WM, WN, stages>;
+    const hipError_t e = ensure_dynamic_lds<kernel>(lds);
     if (e != hipSuccess) return e;
     const unsigned blocks = (unsigned)a.tiles_m * (unsigned)a.tiles_n * (unsigned)a.split;
-    hipLaunchKernelGGL((dense_tile_kernel<T, AT, BT, OUT, BM, BN, WM, WN>), dim3(blocks), dim3(WM * WN * 64), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(WM * WN * 64), lds, s, a);
     return hipGetLastError();
+}
+
+template <bool AT, bool BT, DenseOut WHOLE, DenseOut PIECES, int BM, int BN, int WM, int WN>
+inline hipError_t launch_dense_tile_out(hipStream_t s, const DenseTileArgs &a, int f32)
+{
+    if (a.split > 1) return launch_dense_tile<float, AT, BT, PIECES, BM, BN, WM, WN>(s, a);
+    return f32 ? launch_dense_tile<float, AT, BT, WHOLE, BM, BN, WM, WN>(s, a) : launch_dense_tile<__bf16, AT, BT, WHOLE, BM, BN, WM, WN>(s, a);
 }
 
 // the output's kind and the tile's shape at run time
 template <bool AT, bool BT, DenseOut WHOLE, DenseOut PIECES>
-inline hipError_t launch_dense_tile_any(hipStream_t s, const DenseTileArgs &a, bool big, int f32)
+inline hipError_t launch_dense_tile_any(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32)
 {
-    if (big) {
-        if (a.split > 1) return launch_dense_tile<float, AT, BT, PIECES, 256, 256, 2, 4>(s, a);
-        return f32 ? launch_dense_tile<float, AT, BT, WHOLE, 256, 256, 2, 4>(s, a) : launch_dense_tile<__bf16, AT, BT, WHOLE, 256, 256, 2, 4>(s, a);
-    }
-    if (a.split > 1) return launch_dense_tile<float, AT, BT, PIECES, 128, 128, 2, 2>(s, a);
-    return f32 ? launch_dense_tile<float, AT, BT, WHOLE, 128, 128, 2, 2>(s, a) : launch_dense_tile<__bf16, AT, BT, WHOLE, 128, 128, 2, 2>(s, a);
+    if (tile == DENSE_TILE_256) return launch_dense_tile_out<AT, BT, WHOLE, PIECES, 256, 256, 2, 4>(s, a, f32);
+    if (tile == DENSE_TILE_256_128) return launch_dense_tile_out<AT, BT, WHOLE, PIECES, 256, 128, 4, 2>(s, a, f32);
+    return launch_dense_tile_out<AT, BT, WHOLE, PIECES, 128, 128, 2, 2>(s, a, f32);
 }
 
 }  // namespace alpha
