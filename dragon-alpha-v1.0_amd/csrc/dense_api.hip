@@ -153,8 +153,8 @@ int quads_aligned(int type, std::initializer_list<const void *> p, std::initiali
 // ---- workspaces: the same sequence of blocks for the query (base NULL) and the call --------------------------------
 struct ForwardRoom {
     void *X, *W[2];
-    float *partial;
-    size_t partial_bytes, total;
+    float *pieces;
+    size_t piece_bytes, total;
 };
 ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
 {
@@ -163,8 +163,8 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
     if (dense_few_rows_preferred(type == ALPHA_DENSE_F32, gated, N, OC, IC)) return r;   // operands as they are, no pieces
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC));
-    r.partial_bytes = dense_product_partial_bytes(N, OC, IC, parts_of(type), 1, gated);
-    r.partial = ws.take<float>(r.partial_bytes);
+    r.piece_bytes = dense_product_piece_bytes(N, OC, IC, parts_of(type), 1, gated);
+    r.pieces = ws.take<float>(r.piece_bytes);
     r.total = ws.at;
     return r;
 }
@@ -172,8 +172,8 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
 struct BackwardRoom {
     __bf16 *delta;
     void *X, *W[2];
-    float *sums, *partial;
-    size_t partial_bytes, total;
+    float *sums, *pieces;
+    size_t piece_bytes, total;
 };
 BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *base)
 {
@@ -184,12 +184,12 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < pair; i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC));
     r.sums = ws.take<float>(dense_delta_sum_bytes(N, OC, gated));
-    const size_t for_x = dense_product_partial_bytes(N, IC, OC, parts_of(type), pair, 0);
+    const size_t for_x = dense_product_piece_bytes(N, IC, OC, parts_of(type), pair, 0);
     // a gated pair's filter gradients are one stacked product, or one of them alone
-    const size_t for_w = std::max(dense_product_partial_bytes(OC, IC, N, parts_of(type), 1, 0),
-                                  gated ? dense_product_partial_bytes((int)round8(OC) + OC, IC, N, parts_of(type), 1, 0) : (size_t)0);
-    r.partial_bytes = std::max(for_x, for_w);
-    r.partial = ws.take<float>(r.partial_bytes);
+    const size_t for_w = std::max(dense_product_piece_bytes(OC, IC, N, parts_of(type), 1, 0),
+                                  gated ? dense_product_piece_bytes((int)round8(OC) + OC, IC, N, parts_of(type), 1, 0) : (size_t)0);
+    r.piece_bytes = std::max(for_x, for_w);
+    r.pieces = ws.take<float>(r.piece_bytes);
     r.total = ws.at;
     return r;
 }
@@ -224,8 +224,8 @@ int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, i
     p.K = IC;
     p.f32 = type == ALPHA_DENSE_F32;
     p.ep = ep;
-    p.partial = room.partial;
-    p.partial_bytes = room.partial_bytes;
+    p.pieces = room.pieces;
+    p.piece_bytes = room.piece_bytes;
     if (IC > 0) {
         TRY(operand(fn, s, type, X, ldX, N, IC, room.X, !in_place(type, X, ldX, IC), p.A, 0));
         const bool pack = !in_place(type, W, ldW, IC) || (gated && (!in_place(type, W2, ldW2, IC) || ldW != ldW2));
@@ -286,8 +286,8 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
     DenseProduct p{};
     p.parts = parts_of(type);
     p.f32 = d.f32;
-    p.partial = room.partial;
-    p.partial_bytes = room.partial_bytes;
+    p.pieces = room.pieces;
+    p.piece_bytes = room.piece_bytes;
     if (want_x) {   // deltaX[n, ic] = sum over oc (and over both filters)
         p.A = delta;
         p.sources = pair;

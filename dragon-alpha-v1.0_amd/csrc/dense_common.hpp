@@ -10,28 +10,64 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 // ---- activations ---------------------------------------------------------------------------------------------------
+// exp(-z) from the hardware's 2^x: z log2(e) as a rounded product and its remainder, the remainder applied to first order;
+// within a few units of 2^-24, 2^x's own error among them. 1 / (1 + inf) = 0 from the hardware's reciprocal (2^-23).
+static __device__ __forceinline__ float dense_exp(float z)
+{
+    const float t = z * 1.44269504f, r = fmaf(z, 1.44269504f, -t) + z * 1.925963e-8f;
+    const float p = __builtin_amdgcn_exp2f(t);
+    return fabsf(t) < 126.f ? fmaf(p, r * 0.69314718f, p) : p;   // (beyond: near 0 or infinity, and r may be no number)
+}
+static __device__ __forceinline__ float dense_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + dense_exp(-z)); }
+
+// P(z) = (1 + erf(z / sqrt 2)) / 2 and, where wanted, its derivative D(z) = exp(-z^2 / 2) / sqrt(2 pi). fp32: the library's
+// erf. bf16 (T): erf by Abramowitz and Stegun's formula 7.1.26, within 1.5e-7, with the same exponential as the derivative -
+// a third of the instructions, in kernels that they bound.
+template <typename T>
+static __device__ __forceinline__ float dense_normal(float z, float &density)
+{
+    if constexpr (sizeof(T) == 4) {
+        density = 0.39894228f * expf(-0.5f * z * z);
+        return 0.5f * (1.f + erff(z * 0.70710678f));
+    } else {
+        const float x = fabsf(z) * 0.70710678f, g = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+        const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        density = 0.39894228f * g;
+        const float tail = 0.5f * q * g;                 // P(-|z|)
+        return z < 0.f ? tail : 1.f - tail;
+    }
+}
+
+template <typename T>
 static __device__ __forceinline__ float dense_act(int act, float z, float k)
 {
+    float density;
     switch (act) {   // uniform
     case ALPHA_DENSE_ACT_LEAKY_RELU: return z > 0.f ? z : z * k;
-    case ALPHA_DENSE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case ALPHA_DENSE_ACT_SILU: return z / (1.f + expf(-z));
-    case ALPHA_DENSE_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
+    case ALPHA_DENSE_ACT_GELU: return z * dense_normal<T>(z, density);
+    case ALPHA_DENSE_ACT_SILU: return z * dense_sigmoid(z);
+    case ALPHA_DENSE_ACT_SIGMOID: return dense_sigmoid(z);
     default: return z;
     }
 }
 
+template <typename T>
 static __device__ __forceinline__ float dense_act_slope(int act, float z, float k)
 {
     switch (act) {
     case ALPHA_DENSE_ACT_LEAKY_RELU: return z > 0.f ? 1.f : k;
-    case ALPHA_DENSE_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case ALPHA_DENSE_ACT_GELU: {
+        float density;
+        const float p = dense_normal<T>(z, density);
+        return fmaf(z, density, p);
+    }
     case ALPHA_DENSE_ACT_SILU: {
-        const float s = 1.f / (1.f + expf(-z));
-        return s * (1.f + z * (1.f - s));
+        const float s = dense_sigmoid(z);
+        return s * fmaf(z, 1.f - s, 1.f);
     }
     case ALPHA_DENSE_ACT_SIGMOID: {
-        const float s = 1.f / (1.f + expf(-z));
+        const float s = dense_sigmoid(z);
         return s * (1.f - s);
     }
     default: return 1.f;
@@ -110,10 +146,10 @@ struct DenseProduct {
     int K;
     int f32;              // output type
     DenseEpilogue ep;
-    float *partial;       // room for partial sums, `partial_bytes`
-    size_t partial_bytes;
+    float *pieces;        // room for the pieces of cut reductions, `piece_bytes`
+    size_t piece_bytes;
 };
-size_t dense_product_partial_bytes(int M, int N, int K, int parts, int sources, int gated);
+size_t dense_product_piece_bytes(int M, int N, int K, int parts, int sources, int gated);
 double dense_product_us(int M, int N, int K, int parts, int sources, int gated);   // the plan's estimate
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p);
 

@@ -28,25 +28,25 @@ static __device__ __forceinline__ void run_store(T *p, const float (&v)[R])
         for (int i = 0; i < R; i += 4) quad_store(p + i, floatx4{v[i], v[i + 1], v[i + 2], v[i + 3]});
     }
 }
-template <int R>
+template <typename T, int R>
 static __device__ __forceinline__ void run_act(int act, float (&v)[R], float k)
 {
     switch (act) {   // one branch for the run
     case ALPHA_DENSE_ACT_LEAKY_RELU:
 #pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_LEAKY_RELU, v[e], k);
+        for (int e = 0; e < R; e++) v[e] = dense_act<T>(ALPHA_DENSE_ACT_LEAKY_RELU, v[e], k);
         break;
     case ALPHA_DENSE_ACT_GELU:
 #pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_GELU, v[e], k);
+        for (int e = 0; e < R; e++) v[e] = dense_act<T>(ALPHA_DENSE_ACT_GELU, v[e], k);
         break;
     case ALPHA_DENSE_ACT_SILU:
 #pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_SILU, v[e], k);
+        for (int e = 0; e < R; e++) v[e] = dense_act<T>(ALPHA_DENSE_ACT_SILU, v[e], k);
         break;
     case ALPHA_DENSE_ACT_SIGMOID:
 #pragma unroll
-        for (int e = 0; e < R; e++) v[e] = dense_act(ALPHA_DENSE_ACT_SIGMOID, v[e], k);
+        for (int e = 0; e < R; e++) v[e] = dense_act<T>(ALPHA_DENSE_ACT_SIGMOID, v[e], k);
         break;
     default: break;
     }
@@ -82,7 +82,7 @@ static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, flo
                 if (n + e < N) dense_store(Z + m * ep.ldZ + n + e, v[e]);
         }
     }
-    run_act(ep.act, v, ep.slope);
+    run_act<T>(ep.act, v, ep.slope);
     if (res) {
         if constexpr (R % 4 == 0)
             if (whole) run_load(res + m * ep.ldR + n, t);
@@ -133,7 +133,7 @@ static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &e
             }
         }
     }
-    run_act(ep.act, g, ep.slope);
+    run_act<T>(ep.act, g, ep.slope);
 #pragma unroll
     for (int e = 0; e < R; e++) g[e] *= u[e];
     if constexpr (R % 4 == 0)

@@ -5,83 +5,108 @@
 
 namespace alpha {
 
-// Adds the pieces of a cut reduction in their order and applies the epilogue; one thread per four columns.
+// Adds the pieces of the cut tiles in their order and applies the epilogue: eight columns a thread, a workgroup 256 / (BN / 8)
+// rows of a tile (gated: BN / 16 threads a row, eight columns of each filter).
 template <typename T, bool GATED>
-__global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a, long a_row, long a_k, long b_row, long b_k, FastDiv d_quads)
+__global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a, int bm, int bn, long a_row, long a_k, long b_row, long b_k)
 {
-    const long quads = d_quads.d;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < quads * a.M; i += (long)gridDim.x * 256) {
-        const int m = quads * a.M < (1l << 31) ? (int)fdiv((uint32_t)i, d_quads) : (int)(i / quads);
-        const int n = (int)(i - m * quads) * 4;
-        floatx4 v{0.f, 0.f, 0.f, 0.f}, u = v;
-        const float *src = a.partial + (long)m * a.columns + n;
+    const int lanes = bn / (GATED ? 16 : 8), rows = 256 / lanes, per_tile = bm / rows;
+    const int cut = (int)blockIdx.x / per_tile, row = (int)blockIdx.x % per_tile * rows + (int)threadIdx.x / lanes, lane = (int)threadIdx.x % lanes;
+    int tm, tn;
+    tile_at(a.whole + cut, a.tiles_m, a.tiles_n, tm, tn);
+    const long m = (long)tm * bm + row;
+    const int n = tn * (GATED ? bn / 2 : bn) + lane * 8;
+    if (m >= a.M || n >= a.N) return;
+    float v[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = u[e] = 0.f;
+    // gated: of every 64 columns of a tile 32 are the gate's, the other 32 the other filter's
+    const float *src = a.pieces + ((long)cut * bm + row) * bn + (GATED ? lane / 4 * 64 + lane % 4 * 8 : lane * 8);
+    const long step = ((long)a.tiles_m * a.tiles_n - a.whole) * bm * bn;
 #pragma unroll 4
-        for (int p = 0; p < a.split; p++, src += (long)a.M * a.columns) {
-            if ((a.columns & 3) == 0 && (a.N & 3) == 0) {
-                v += *reinterpret_cast<const floatx4 *>(src);
-                if (GATED) u += *reinterpret_cast<const floatx4 *>(src + a.N);
-            } else {
+    for (int p = 0; p < a.split; p++, src += step) {
+        float t[8];
+        run_load(src, t);
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (n + e < a.N) {
-                        v[e] += src[e];
-                        if (GATED) u[e] += src[a.N + e];
-                    }
-            }
-        }
-        if constexpr (__is_same(T, float)) {
+        for (int e = 0; e < 8; e++) v[e] += t[e];
+        if constexpr (GATED) {
+            run_load(src + 32, t);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (n + e >= a.N) break;
-                if (v[e] != v[e])
-                    v[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[0], a.B[1], (n + e) * b_row, b_k, a.planeB,
-                                         GATED ? 1 : a.combos / a.parts6, a.K);
-                if (GATED && u[e] != u[e])
-                    u[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[1], a.B[1], (n + e) * b_row, b_k, a.planeB, 1, a.K);
-            }
+            for (int e = 0; e < 8; e++) u[e] += t[e];
         }
-        float x[4] = {v[0], v[1], v[2], v[3]}, y[4] = {u[0], u[1], u[2], u[3]};
-        if constexpr (GATED) dense_finish_gated<T>(a.ep, x, y, m, n, a.N);
-        else dense_finish<T>(a.ep, x, m, n, a.N);
     }
+    if constexpr (__is_same(T, float)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (n + e >= a.N) break;
+            if (v[e] != v[e])
+                v[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[0], a.B[1], (n + e) * b_row, b_k, a.planeB,
+                                     GATED ? 1 : a.combos / a.parts6, a.K);
+            if (GATED && u[e] != u[e])
+                u[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[1], a.B[1], (n + e) * b_row, b_k, a.planeB, 1, a.K);
+        }
+    }
+    if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n, a.N);
+    else dense_finish<T>(a.ep, v, m, n, a.N);
 }
 
 namespace {
 
 struct Plan {
     DenseTile tile;
-    int split, per, tiles_m, tiles_n, steps;
+    int tiles_m, tiles_n, whole, split, per, steps;
     double us;
 };
 
-// Tile shape and cut of the reduction: the least of an estimate of the device's time, its constants measured on NT products
-// of 256 x 256 x 256 to 8192 x 4096 x 4096 (a workgroup's step with the device nearly empty and full, 256 / 256 x 128 / 128:
-// 0.57 / 0.34 / 0.36 and 0.72 / 0.48 / 0.59 us, the last with two workgroups on a compute unit). `room`: bytes for the pieces.
+size_t piece_bytes(const Plan &p) { return ((size_t)p.tiles_m * p.tiles_n - p.whole) * p.split * DENSE_TILE_M[p.tile] * DENSE_TILE_N[p.tile] * 4; }
+
+// Tile shape and cut: whole tiles for as many rounds as the device's workgroup slots go into, and the tiles that are left (or
+// all, where there are few) with their reduction cut so that they fill the device once more. The choice is the least of an
+// estimate of the device's time; its constants were measured on products of 256 x 256 x 256 to 8192 x 4096 x 4096: a
+// workgroup's step with the device nearly empty and full, 256 / 256 x 128 / 128: 0.57 / 0.34 / 0.36 and 0.70 / 0.48 / 0.59 us,
+// the last with two workgroups on a compute unit.
 Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t room)
 {
-    static constexpr double empty[DENSE_TILES] = {0.57, 0.34, 0.36}, full[DENSE_TILES] = {0.72, 0.48, 0.59}, fixed[DENSE_TILES] = {6.5, 5.0, 3.0};
+    static constexpr double empty[DENSE_TILES] = {0.57, 0.34, 0.36}, full[DENSE_TILES] = {0.70, 0.48, 0.59}, fixed[DENSE_TILES] = {6.5, 5.0, 3.0};
     const int cus = std::max(1, device_cu_count());
     const int nk = std::max(1, (K + 31) / 32), combos = (parts == 3 ? 6 : 1) * sources, steps = nk * combos;
-    const double outputs = (double)M * N * (gated ? 2 : 1), bytes_per_us = 4.2e6;
+    const double bytes_per_us = 4.2e6, outputs = (double)M * N * (gated ? 2 : 1);
     Plan best{};
     best.us = 1e30;
-    for (int tile = 0; tile < DENSE_TILES; tile++) {
-        const int bm = DENSE_TILE_M[tile], bn = DENSE_TILE_N[tile] / (gated ? 2 : 1);
-        const int tm = (int)(((long)M + bm - 1) / bm), tn = (N + bn - 1) / bn;
-        const long tiles = (long)tm * tn;
-        for (int split = 1; split <= 64; split++) {
+    for (int t = 0; t < DENSE_TILES; t++) {
+        const int bm = DENSE_TILE_M[t], bn = DENSE_TILE_N[t];
+        Plan p{};
+        p.tile = (DenseTile)t;
+        p.tiles_m = (int)(((long)M + bm - 1) / bm);
+        p.tiles_n = (N * (gated ? 2 : 1) + bn - 1) / bn;
+        p.steps = steps;
+        const long tiles = (long)p.tiles_m * p.tiles_n;
+        // time of `groups` workgroups of `per` steps each
+        auto rounds_us = [&](long groups, int per) {
+            const bool pairs = t == DENSE_TILE_128 && groups > cus;
+            const long slots = pairs ? 2l * cus : cus, rounds = (groups + slots - 1) / slots;
+            const double filled = std::min(1.0, (double)groups / slots);
+            return rounds * (per * (t == DENSE_TILE_128 ? (pairs ? full[t] : empty[t]) : empty[t] + (full[t] - empty[t]) * filled) + fixed[t]);
+        };
+        auto consider = [&](long whole, int split) {
             // whole k steps: a piece holds all parts of its products, so none leaves fp32's range that the sum would not
             // (and an even number of steps: the kernel's loop does two at a time)
-            const int per = (nk + 2 * split - 1) / (2 * split) * 2 * combos;
-            if (split > 1 && (per < 8 || split * outputs * 4 > (double)room)) break;
-            if ((steps + per - 1) / per != split) continue;   // every piece has a step
-            const long groups = tiles * split;
-            const bool pairs = tile == DENSE_TILE_128 && groups > cus;
-            const long slots = pairs ? 2l * cus : cus, rounds = (groups + slots - 1) / slots;
-            const double fill = std::min(1.0, (double)groups / slots);
-            double us = 3.5 + rounds * (per * (tile == DENSE_TILE_128 ? (pairs ? full[tile] : empty[tile]) : empty[tile] + (full[tile] - empty[tile]) * fill) + fixed[tile]);
-            us += split > 1 ? 5.0 + outputs * (8.0 * split + 2) / bytes_per_us : outputs * (parts == 3 ? 4 : 2) / bytes_per_us;
-            if (us < best.us) best = Plan{(DenseTile)tile, split, per, tm, tn, steps, us};
+            p.whole = (int)whole;
+            p.split = split;
+            p.per = (nk + 2 * split - 1) / (2 * split) * 2 * combos;
+            const long left = tiles - whole;
+            p.us = 3.5 + outputs * (parts == 3 ? 4 : 2) / bytes_per_us + (whole > 0 ? rounds_us(whole, steps) : 0.0);
+            if (left > 0) {
+                if (split < 2 || p.per < 8 || (steps + p.per - 1) / p.per != split || piece_bytes(p) > room) return;   // (every piece has a step)
+                p.us += rounds_us(left * split, p.per) + 4.5 + piece_bytes(p) * 2.0 / bytes_per_us;
+            }
+            if (p.us < best.us) best = p;
+        };
+        consider(tiles, 1);
+        const long slots = t == DENSE_TILE_128 ? 2l * cus : cus, starts[2] = {0, tiles / slots * slots};
+        for (int i = 0; i < 2; i++) {
+            if ((i == 1 && starts[1] == 0) || starts[i] == tiles || tiles - starts[i] > slots) continue;
+            for (int split = 2; split <= 64; split += split < 8 ? 1 : split < 16 ? 2 : 8) consider(starts[i], split);
         }
     }
     return best;
@@ -89,11 +114,10 @@ Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t ro
 
 }  // namespace
 
-size_t dense_product_partial_bytes(int M, int N, int K, int parts, int sources, int gated)
+size_t dense_product_piece_bytes(int M, int N, int K, int parts, int sources, int gated)
 {
     // as many pieces as the plan without a limit takes
-    const Plan p = make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60);
-    return p.split > 1 ? (size_t)p.split * M * N * (gated ? 2 : 1) * 4 : 0;
+    return piece_bytes(make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60));
 }
 
 double dense_product_us(int M, int N, int K, int parts, int sources, int gated) { return make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60).us; }
@@ -101,7 +125,7 @@ double dense_product_us(int M, int N, int K, int parts, int sources, int gated) 
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
 {
     if (p.M <= 0 || p.N <= 0) return hipSuccess;
-    const Plan plan = make_plan(p.M, p.N, p.K, p.parts, p.sources, p.gated, p.partial ? p.partial_bytes : 0);
+    const Plan plan = make_plan(p.M, p.N, p.K, p.parts, p.sources, p.gated, p.pieces ? p.piece_bytes : 0);
     DenseTileArgs a{};
     for (int i = 0; i < 2; i++) {
         a.A[i] = p.A.p[i];
@@ -117,29 +141,28 @@ hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
     a.parts6 = p.parts == 3 ? 6 : 1;
     a.combos = a.parts6 * p.sources;
     a.steps = plan.steps;
+    a.whole = plan.whole;
     a.split = plan.split;
     a.per = plan.per;
     a.tiles_m = plan.tiles_m;
     a.tiles_n = plan.tiles_n;
     a.ep = p.ep;
-    a.partial = p.partial;
-    a.columns = p.gated ? 2 * p.N : p.N;
+    a.pieces = p.pieces;
     hipError_t e;
     if (p.a_t) e = launch_dense_tile_tt(s, a, plan.tile, p.f32);
     else if (p.b_t) e = launch_dense_tile_st(s, a, plan.tile, p.f32);
     else if (p.gated) e = launch_dense_tile_gated(s, a, plan.tile, p.f32);
     else e = launch_dense_tile_ss(s, a, plan.tile, p.f32);
-    if (e != hipSuccess || a.split == 1) return e;
-    const long quads = (p.N + 3) / 4, work = quads * p.M;
-    const FastDiv d = make_fastdiv((uint32_t)quads);
-    const dim3 grid((unsigned)std::min<long>((work + 255) / 256, 8192));
+    const int bm = DENSE_TILE_M[plan.tile], bn = DENSE_TILE_N[plan.tile], cut = plan.tiles_m * plan.tiles_n - plan.whole;
+    if (e != hipSuccess || cut == 0) return e;
+    const dim3 grid((unsigned)cut * (unsigned)(bm * bn / (p.gated ? 16 : 8) / 256));
     const long a_row = p.a_t ? 1 : p.A.ld, a_k = p.a_t ? p.A.ld : 1, b_row = p.b_t ? 1 : p.B.ld, b_k = p.b_t ? p.B.ld : 1;
     if (p.gated) {
-        if (p.f32) hipLaunchKernelGGL((dense_pieces_kernel<float, true>), grid, dim3(256), 0, s, a, a_row, a_k, b_row, b_k, d);
-        else hipLaunchKernelGGL((dense_pieces_kernel<__bf16, true>), grid, dim3(256), 0, s, a, a_row, a_k, b_row, b_k, d);
+        if (p.f32) hipLaunchKernelGGL((dense_pieces_kernel<float, true>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
+        else hipLaunchKernelGGL((dense_pieces_kernel<__bf16, true>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
     } else {
-        if (p.f32) hipLaunchKernelGGL((dense_pieces_kernel<float, false>), grid, dim3(256), 0, s, a, a_row, a_k, b_row, b_k, d);
-        else hipLaunchKernelGGL((dense_pieces_kernel<__bf16, false>), grid, dim3(256), 0, s, a, a_row, a_k, b_row, b_k, d);
+        if (p.f32) hipLaunchKernelGGL((dense_pieces_kernel<float, false>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
+        else hipLaunchKernelGGL((dense_pieces_kernel<__bf16, false>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
     }
     return hipGetLastError();
 }

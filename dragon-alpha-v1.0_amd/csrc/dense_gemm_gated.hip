@@ -5,7 +5,7 @@ namespace alpha {
 
 hipError_t launch_dense_tile_gated(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32)
 {
-    return launch_dense_tile_any<false, false, DENSE_GATED, DENSE_PARTIAL_GATED>(s, a, tile, f32);
+    return launch_dense_tile_any<false, false, true>(s, a, tile, f32);
 }
 
 }  // namespace alpha

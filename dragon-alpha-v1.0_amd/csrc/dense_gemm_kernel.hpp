@@ -31,15 +31,27 @@ struct DenseTileArgs {
     int combos;        // products per 32 k: parts (1 or 6) x sources
     int parts6;        // 6 for the three-part split, else 1
     int steps;         // combos for every 32 k
-    int split, per;    // the reduction is cut into `split` runs of `per` steps (an even number)
     int tiles_m, tiles_n;
+    int whole;         // the first `whole` tiles are a workgroup's whole work; the others' reductions are cut
+    int split, per;    // into `split` runs of `per` steps (an even number)
     DenseEpilogue ep;
-    float *partial;    // [split][M][columns of C]
-    int columns;       // N, or 2 N where gated (gate columns first)
+    float *pieces;     // [split][tiles - whole][BM][BN], as the tile kernel has them
 };
 
-// what leaves the kernel
-enum DenseOut { DENSE_PLAIN, DENSE_GATED, DENSE_PARTIAL, DENSE_PARTIAL_GATED };
+// The XCD-aware order of tiles. Workgroups go round the eight XCDs, so every eighth one shares an L2: an XCD gets a contiguous
+// run of `count` places.
+static __device__ __forceinline__ int xcd_place(int id, int count)
+{
+    const int each = count / 8, more = count % 8, xcd = id & 7;
+    return xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+}
+// Tile number -> tile row and column: panels of 8 tile rows, so that a run of tiles reuses both operands out of the L2.
+static __device__ __forceinline__ void tile_at(int tile, int tiles_m, int tiles_n, int &tm, int &tn)
+{
+    const int panel = tile / (8 * tiles_n), first = panel * 8, deep = tiles_m - first < 8 ? tiles_m - first : 8, in = tile - panel * 8 * tiles_n;
+    tm = first + in % deep;
+    tn = in / deep;
+}
 
 static __device__ __forceinline__ void load_to_lds(unsigned lds, unsigned voffset, uintx4 rsrc)
 {
@@ -103,13 +115,12 @@ static __device__ __forceinline__ int t_permutation(int k) { return ((k & 3) | (
 // four groups of rows must come to four different chunks: 0, 3, 2, 1 for g = 0 .. 3. Counted: no conflicts.
 static __device__ __forceinline__ int s_permutation(int g) { return (g & 1) | ((g ^ (g >> 1)) & 1) << 1; }
 
-template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN, int STAGES>
+template <typename T, bool AT, bool BT, bool GATED, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const DenseTileArgs a)
 {
     constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
     constexpr int LA = BM * 4 / NT, LB = BN * 4 / NT;       // 16-byte loads of a thread per step
     constexpr unsigned ABYTES = BM * 64, BBYTES = BN * 64, STAGE = ABYTES + BBYTES, RING = STAGES * STAGE;
-    constexpr bool GATED = OUT == DENSE_GATED || OUT == DENSE_PARTIAL_GATED;
     static_assert(TM % 16 == 0 && TN % 64 == 0 && LA >= 1 && LB >= 1 && NT % 256 == 0, "tile shape");
     extern __shared__ char smem[];
 
@@ -117,20 +128,17 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    // The tile: workgroups go round the eight XCDs, so every eighth one shares an L2; an XCD gets a contiguous run of tiles,
-    // ordered in panels of 8 tile rows so that the run reuses both operands out of that L2.
-    const int tiles = a.tiles_m * a.tiles_n;
-    int id = blockIdx.x, piece = 0;
-    {
-        const int total = tiles * a.split, each = total / 8, more = total % 8, xcd = id & 7, at = id >> 3;
-        id = xcd * each + (xcd < more ? xcd : more) + at;
+    const int cut_tiles = a.tiles_m * a.tiles_n - a.whole;
+    const bool cut = (int)blockIdx.x >= a.whole;
+    int piece = 0, tile, tm, tn;
+    if (cut) {   // piece by piece over all cut tiles: neighbours read the same k
+        const int at = xcd_place((int)blockIdx.x - a.whole, cut_tiles * a.split);
+        piece = at / cut_tiles;
+        tile = a.whole + at % cut_tiles;
+    } else {
+        tile = xcd_place((int)blockIdx.x, a.whole);
     }
-    if (a.split > 1) {
-        piece = id / tiles;
-        id -= piece * tiles;
-    }
-    const int panel = id / (8 * a.tiles_n), first = panel * 8, deep = a.tiles_m - first < 8 ? a.tiles_m - first : 8;
-    const int tm = first + (id - panel * 8 * a.tiles_n) % deep, tn = (id - panel * 8 * a.tiles_n) / deep;
+    tile_at(tile, a.tiles_m, a.tiles_n, tm, tn);
     const int m0 = tm * BM, n0 = tn * (GATED ? BN / 2 : BN);
 
     // ---- where the loads of a step come from: a per-lane offset, the rest in the descriptor ----
@@ -166,7 +174,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     // ---- the steps of this workgroup ----
     const int t0 = piece * a.per;
     int left = a.steps - t0;
-    if (left > a.per) left = a.per;
+    if (cut && left > a.per) left = a.per;
     int combo = t0 % a.combos;                         // of the next step to load
     int krem = a.K - t0 / a.combos * 32;               // k from its first on; <= 0: nothing, zeros
     const long stepA = AT ? 32 * a.ldA : 32, stepB = BT ? 32 * a.ldB : 32;
@@ -336,19 +344,10 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
             run_load(part + row * ROW + at, v);
             if constexpr (GATED) run_load(part + row * ROW + 32 + at, u);
             if (m >= a.M || n >= a.N) continue;
-            if constexpr (OUT == DENSE_PARTIAL || OUT == DENSE_PARTIAL_GATED) {
-                float *dst = a.partial + (piece * (long)a.M + m) * a.columns + n;
-                if ((a.N & 3) == 0 && n + 8 <= a.N) {
-                    run_store(dst, v);
-                    if constexpr (GATED) run_store(dst + a.N, u);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (n + e < a.N) {
-                            dst[e] = v[e];
-                            if constexpr (GATED) dst[a.N + e] = u[e];
-                        }
-                }
+            if (cut) {
+                float *dst = a.pieces + (((long)piece * cut_tiles + (tile - a.whole)) * BM + (wm * TM + i * 16 + row)) * BN + wn * TN + at;
+                run_store(dst, v);
+                if constexpr (GATED) run_store(dst + 32, u);
             } else {
                 if constexpr (__is_same(T, float)) {
                     float sum = 0.f;
@@ -365,7 +364,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
         }
         wave_fence();
     }
-    if constexpr (__is_same(T, float) && (OUT == DENSE_PLAIN || OUT == DENSE_GATED)) {
+    if constexpr (__is_same(T, float)) {
         static_assert(MF / 2 * TURNS <= 32, "one bit per run");
         while (again) {
             const int bit = __ffs(again) - 1;

@@ -14,33 +14,28 @@ hipError_t launch_dense_tile_gated(hipStream_t s, const DenseTileArgs &a, DenseT
 hipError_t launch_dense_tile_st(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32);      // B with k as its rows
 hipError_t launch_dense_tile_tt(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32);      // both with k as their rows
 
-template <typename T, bool AT, bool BT, DenseOut OUT, int BM, int BN, int WM, int WN>
+template <typename T, bool AT, bool BT, bool GATED, int BM, int BN, int WM, int WN>
 inline hipError_t launch_dense_tile(hipStream_t s, const DenseTileArgs &a)
 {
     constexpr int stages = 4;
     constexpr size_t lds = stages * (BM + BN) * 64;
-    constexpr auto kernel = dense_tile_kernel<T, AT, BT, OUT, BM, BN, WM, WN, stages>;
+    constexpr auto kernel = dense_tile_kernel<T, AT, BT, GATED, BM, BN, WM, WN, stages>;
     const hipError_t e = ensure_dynamic_lds<kernel>(lds);
     if (e != hipSuccess) return e;
-    const unsigned blocks = (unsigned)a.tiles_m * (unsigned)a.tiles_n * (unsigned)a.split;
+    const unsigned blocks = (unsigned)a.whole + ((unsigned)a.tiles_m * (unsigned)a.tiles_n - (unsigned)a.whole) * (unsigned)a.split;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(WM * WN * 64), lds, s, a);
     return hipGetLastError();
 }
 
-template <bool AT, bool BT, DenseOut WHOLE, DenseOut PIECES, int BM, int BN, int WM, int WN>
-inline hipError_t launch_dense_tile_out(hipStream_t s, const DenseTileArgs &a, int f32)
-{
-    if (a.split > 1) return launch_dense_tile<float, AT, BT, PIECES, BM, BN, WM, WN>(s, a);
-    return f32 ? launch_dense_tile<float, AT, BT, WHOLE, BM, BN, WM, WN>(s, a) : launch_dense_tile<__bf16, AT, BT, WHOLE, BM, BN, WM, WN>(s, a);
-}
-
-// the output's kind and the tile's shape at run time
-template <bool AT, bool BT, DenseOut WHOLE, DenseOut PIECES>
+// the output's type and the tile's shape at run time
+template <bool AT, bool BT, bool GATED>
 inline hipError_t launch_dense_tile_any(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32)
 {
-    if (tile == DENSE_TILE_256) return launch_dense_tile_out<AT, BT, WHOLE, PIECES, 256, 256, 2, 4>(s, a, f32);
-    if (tile == DENSE_TILE_256_128) return launch_dense_tile_out<AT, BT, WHOLE, PIECES, 256, 128, 4, 2>(s, a, f32);
-    return launch_dense_tile_out<AT, BT, WHOLE, PIECES, 128, 128, 2, 2>(s, a, f32);
+    switch (tile) {
+    case DENSE_TILE_256: return f32 ? launch_dense_tile<float, AT, BT, GATED, 256, 256, 2, 4>(s, a) : launch_dense_tile<__bf16, AT, BT, GATED, 256, 256, 2, 4>(s, a);
+    case DENSE_TILE_256_128: return f32 ? launch_dense_tile<float, AT, BT, GATED, 256, 128, 4, 2>(s, a) : launch_dense_tile<__bf16, AT, BT, GATED, 256, 128, 4, 2>(s, a);
+    default: return f32 ? launch_dense_tile<float, AT, BT, GATED, 128, 128, 2, 2>(s, a) : launch_dense_tile<__bf16, AT, BT, GATED, 128, 128, 2, 2>(s, a);
+    }
 }
 
 }  // namespace alpha

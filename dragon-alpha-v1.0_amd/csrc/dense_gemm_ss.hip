@@ -5,7 +5,7 @@ namespace alpha {
 
 hipError_t launch_dense_tile_ss(hipStream_t s, const DenseTileArgs &a, DenseTile tile, int f32)
 {
-    return launch_dense_tile_any<false, false, DENSE_PLAIN, DENSE_PARTIAL>(s, a, tile, f32);
+    return launch_dense_tile_any<false, false, false>(s, a, tile, f32);
 }
 
 }  // namespace alpha

@@ -9,14 +9,22 @@ namespace alpha {
 
 namespace {
 
-// Eight consecutive elements of a row, c .. c+7 of `cols`; the rest zeros. VEC: 16-byte loads are possible.
+// Eight consecutive elements of a row, c .. c+7 of `cols`; the rest zeros. VEC: rows begin at multiples of four elements (128-bit
+// loads take an 8-byte address).
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T *row, int c, int cols, float (&v)[8])
 {
     if (VEC && c + 8 <= cols) {
-        const floatx4 lo = quad_load(row + c), hi = quad_load(row + c + 4);
+        if constexpr (sizeof(T) == 2) {
+            bf16x8 t;
+            __builtin_memcpy(&t, __builtin_assume_aligned(row + c, 8), 16);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = lo[e], v[4 + e] = hi[e];
+            for (int e = 0; e < 8; e++) v[e] = (float)t[e];
+        } else {
+            const floatx4 lo = quad_load(row + c), hi = quad_load(row + c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = lo[e], v[4 + e] = hi[e];
+        }
         return;
     }
 #pragma unroll
@@ -99,10 +107,10 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, lo
                 if (c + e >= d.cols) {   // pad columns: zeros, whatever act(0) is
                     dy[e] = out2[e] = 0.f;
                 } else if constexpr (GATED) {
-                    out2[e] = dy[e] * dense_act(d.act, z[e], d.slope);
-                    dy[e] *= u[e] * dense_act_slope(d.act, z[e], d.slope);
+                    out2[e] = dy[e] * dense_act<T>(d.act, z[e], d.slope);
+                    dy[e] *= u[e] * dense_act_slope<T>(d.act, z[e], d.slope);
                 } else if (d.act != ALPHA_DENSE_ACT_NONE) {
-                    dy[e] *= dense_act_slope(d.act, z[e], d.slope);
+                    dy[e] *= dense_act_slope<T>(d.act, z[e], d.slope);
                 }
                 sum[e] += dy[e];
                 if constexpr (GATED) sum2[e] += out2[e];
@@ -138,6 +146,7 @@ __global__ __launch_bounds__(256) void dense_delta_sum_kernel(const float *__res
     const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4, col = blockIdx.x * 16 + cx;
     float t = 0.f;
     if (col < cols)
+#pragma unroll 4
         for (int r = ry; r < runs; r += 16) t += sums[((long)r * of + which) * cols + col];
     part[ry][cx] = t;
     __syncthreads();
@@ -151,11 +160,11 @@ __global__ __launch_bounds__(256) void dense_delta_sum_kernel(const float *__res
 
 namespace {
 
-// Runs of rows: enough workgroups for the device, at least 32 rows each (a run costs a row of sums), at most 512 runs.
+// Runs of rows: enough workgroups for the device, at least 32 rows each (a run costs a row of sums), at most 256 runs.
 long delta_rows_per(long rows, int cols)
 {
     const long blocks_x = (cols + 255) / 256, want = std::max<long>(1, 2048 / std::max<long>(1, blocks_x));
-    const long runs = std::min<long>(512, std::max<long>(1, std::min(want, rows / 32)));
+    const long runs = std::min<long>(256, std::max<long>(1, std::min(want, rows / 32)));
     return std::max<long>(1, (rows + runs - 1) / runs);
 }
 

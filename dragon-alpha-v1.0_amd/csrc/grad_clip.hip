@@ -3,7 +3,7 @@
 // call returns, and a captured graph holds its own copy).
 //
 // Squares are summed in fp64: exact to the last bit of a long sum, and neither 1e-25 nor 1e+25 leaves the range. A
-// workgroup takes pieces of PIECE elements of any tensor; its partial sum goes to its own word, and the short kernel
+// workgroup takes a piece of one tensor; its partial sum goes to its own word, and the short kernel
 // adds the words in a fixed order, so the norm's bits do not change from run to run.
 #include "dense_common.hpp"
 
@@ -19,8 +19,9 @@ struct GradTensors {
     int first_piece[SLOTS + 1];   // pieces of tensor i: first_piece[i] .. first_piece[i + 1] - 1 of the launch
     unsigned char f32[SLOTS];
     int count;
+    int piece;                    // elements of a piece
 };
-constexpr int PIECE = 16384;
+constexpr int PIECE = 16384, MORE = 4;   // a piece, or MORE of them where there are many
 
 namespace {
 
@@ -50,7 +51,7 @@ __device__ __forceinline__ double piece_squares(const T *p, int n)
     }
     const int vectors = (n - head) / V;
     const vec *q = reinterpret_cast<const vec *>(p + head);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = threadIdx.x; i < vectors; i += 256) {
         const vec v = q[i];
 #pragma unroll
@@ -109,22 +110,28 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const GradTensors t, 
 {
     __shared__ double lds[4];
     const int i = tensor_of(t, blockIdx.x);
-    const long at = (long)(blockIdx.x - t.first_piece[i]) * PIECE;
-    const int n = (int)(t.length[i] - at < PIECE ? t.length[i] - at : PIECE);
+    const long at = (long)(blockIdx.x - t.first_piece[i]) * t.piece;
+    const int n = (int)(t.length[i] - at < t.piece ? t.length[i] - at : t.piece);
     const double v = t.f32[i] ? piece_squares(static_cast<const float *>(t.src[i]) + at, n)
                               : piece_squares(static_cast<const __bf16 *>(t.src[i]) + at, n);
     const double sum = workgroup_sum(v, lds);
     if (threadIdx.x == 0) words[blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(const double *__restrict__ words, long count, float max_norm, float eps, float *__restrict__ norm_c)
+__global__ __launch_bounds__(1024) void grad_norm_kernel(const double *__restrict__ words, long count, float max_norm, float eps, float *__restrict__ norm_c)
 {
-    __shared__ double lds[4];
+    __shared__ double lds[16];
     double v = 0.0;
-    for (long i = threadIdx.x; i < count; i += 256) v += words[i];
-    const double norm = sqrt(workgroup_sum(v, lds));
+#pragma unroll 4
+    for (long i = threadIdx.x; i < count; i += 1024) v += words[i];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_down(v, d, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
     if (threadIdx.x == 0) {
-        const double c = (double)max_norm / (norm + (double)eps);
+        v = 0.0;
+        for (int i = 0; i < 16; i++) v += lds[i];
+        const double norm = sqrt(v), c = (double)max_norm / (norm + (double)eps);
         norm_c[0] = (float)norm;
         norm_c[1] = c < 1.0 || c != c ? (float)c : 1.f;
     }
@@ -135,23 +142,30 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const GradTensors t, co
     const int i = tensor_of(t, blockIdx.x);
     const float c = norm_c[1];
     if (c == 1.f && t.src[i] == t.dst[i]) return;
-    const long at = (long)(blockIdx.x - t.first_piece[i]) * PIECE;
-    const int n = (int)(t.length[i] - at < PIECE ? t.length[i] - at : PIECE);
+    const long at = (long)(blockIdx.x - t.first_piece[i]) * t.piece;
+    const int n = (int)(t.length[i] - at < t.piece ? t.length[i] - at : t.piece);
     if (t.f32[i]) piece_scale(static_cast<const float *>(t.src[i]) + at, static_cast<float *>(t.dst[i]) + at, n, c);
     else piece_scale(static_cast<const __bf16 *>(t.src[i]) + at, static_cast<__bf16 *>(t.dst[i]) + at, n, c);
 }
 
-long grad_pieces(long length) { return (length + PIECE - 1) / PIECE; }
+long grad_pieces(long length)   // at most
+{
+    return (length + PIECE - 1) / PIECE;
+}
 
 hipError_t launch_grad_clip(hipStream_t s, int count, const int *types, const int64_t *lengths, const void *const *src, void *const *dst,
                             float max_norm, float eps, float *norm_c, double *words)
 {
-    long done = 0;
+    long done = 0, total = 0;
+    for (int i = 0; i < count; i++) total += lengths[i];
+    // up to 4096 pieces of the small size are 16 per compute unit; beyond, longer pieces save their beginnings and ends
+    const int piece = total > 4096l * PIECE ? MORE * PIECE : PIECE;
     for (int pass = 0; pass < (dst ? 2 : 1); pass++) {
         int next = 0;
         long offset = 0;   // elements of tensor `next` already dealt with (a launch holds at most 2^30 pieces)
         while (true) {
             GradTensors t{};
+            t.piece = piece;
             long pieces = 0;
             while (next < count && t.count < GradTensors::SLOTS && pieces < (1l << 30)) {
                 const long rest = lengths[next] - offset;
@@ -161,13 +175,13 @@ hipError_t launch_grad_clip(hipStream_t s, int count, const int *types, const in
                     continue;
                 }
                 const long size = types[next] == ALPHA_DENSE_F32 ? 4 : 2;
-                const long take = std::min<long>(rest, ((1l << 30) - pieces) * PIECE);
+                const long take = std::min<long>(rest, ((1l << 30) - pieces) * piece);
                 t.src[t.count] = static_cast<const char *>(src[next]) + offset * size;
                 t.dst[t.count] = dst ? static_cast<char *>(dst[next]) + offset * size : nullptr;
                 t.length[t.count] = take;
                 t.f32[t.count] = types[next] == ALPHA_DENSE_F32;
                 t.first_piece[t.count] = (int)pieces;
-                pieces += grad_pieces(take);
+                pieces += (take + piece - 1) / piece;
                 t.count++;
                 offset += take;
             }
@@ -179,7 +193,7 @@ hipError_t launch_grad_clip(hipStream_t s, int count, const int *types, const in
             if (pass == 0) done += pieces;
         }
         if (pass == 0) {
-            hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, s, words, done, max_norm, eps, norm_c);
+            hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, s, words, done, max_norm, eps, norm_c);
             if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         }
     }

@@ -46,21 +46,11 @@ def _array(kind, values):
     return None if values is None else (kind * max(1, len(values)))(*values)
 
 
-def _call(name, *args):
-    L = _lib()
-    conv = []
-    for c, a in zip(_SIGS[name], args):
-        if c in "Sq":
-            conv.append(_array(_L, a))
-        elif c == "n":
-            conv.append(_array(_I, a))
-        elif c == "t":
-            conv.append(_array(_P, a))
-        else:
-            conv.append(a)
-    rc = getattr(L, name)(*conv)
+def _call(name, streams, *args):
+    """`args` as ctypes takes them for the signature: integers, floats, arrays."""
+    rc = getattr(_lib(), name)((_L * max(1, len(streams)))(*streams), *args)
     if rc != 0:
-        raise native.AlphaConvError("%s failed (%d): %s" % (name, rc, L.alpha_dense_last_error().decode()))
+        raise native.AlphaConvError("%s failed (%d): %s" % (name, rc, native.lib().alpha_dense_last_error().decode()))
 
 
 def _workspace(name, *args):
@@ -130,4 +120,5 @@ class Cuda_dense:
     @staticmethod
     def gradClip(streamArray, length, count, types, lengths, src, dst, max_norm, eps, norm_c, workspace, workspace_bytes):
         """norm_c = {norm, c} with c = min(1, max_norm / (norm + eps)); dst = src * c (dst None: only the norm)."""
-        _call("alpha_gradClip", streamArray, length, count, types, lengths, src, dst, max_norm, eps, norm_c, workspace, workspace_bytes)
+        _call("alpha_gradClip", streamArray, length, count, _array(_I, types), _array(_L, lengths), _array(_P, src), _array(_P, dst),
+              max_norm, eps, norm_c, workspace, workspace_bytes)

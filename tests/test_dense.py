@@ -37,7 +37,7 @@ def test_workspace_queries(query):
 
 def forward(**kw):
     a = dict(streams=[0], length=1, type=D.BF16, X=P, xs=64, W=2 * P, ws=64, B=3 * P, act=D.ACT_GELU, k=0.0, R=4 * P, rs=32, Z=5 * P, zs=32,
-             Y=6 * P, ys=32, N=16, IC=64, OC=32, work=7 * P, bytes=BIG)
+             Y=6 * P, ys=32, N=5000, IC=64, OC=32, work=7 * P, bytes=BIG)
     a.update(kw)
     D.matMul_fused(*a.values())
 
@@ -78,7 +78,7 @@ def test_dmatMul_refusals(change, message):
 ])
 def test_gatedMatMul_refusals(change, message):
     a = dict(streams=[0], length=1, type=D.F32, X=P, xs=64, Wg=2 * P, wgs=64, Bg=0, Wu=3 * P, wus=64, Bu=0, act=D.ACT_SILU, k=0.0,
-             G=4 * P, gs=32, U=5 * P, us=32, H=9 * P, hs=32, N=16, IC=64, OC=32, work=7 * P, bytes=BIG)
+             G=4 * P, gs=32, U=5 * P, us=32, H=9 * P, hs=32, N=5000, IC=64, OC=32, work=7 * P, bytes=BIG)
     a.update(change)
     with pytest.raises(pkg.AlphaConvError, match=message):
         D.gatedMatMul(*a.values())

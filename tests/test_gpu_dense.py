@@ -7,7 +7,10 @@ Tolerances, per element, from the arithmetic:
   sigmas of them. fp32 products leave out parts below 2^-23 of a product each: 8 * 2^-23 S;
 * bf16 backward: deltaZ rounded to bf16 before its products, 2^-8 relative per term, independent: six sigmas of a uniform
   error, 6 / sqrt(3) 2^-8 S;
-* activations: erff / expf good to a few ulps, 2^-20 of max(1, |z|) absolute; the product's own error passes with a slope <= 1.2.
+* activations: exponentials and erf good to a few units of 2^-24, so 2^-20 of max(1, |z|) absolute; the product's own error
+  passes with a slope <= 1.2. Their derivatives are sums of terms of at most max(1, |z|) that may cancel (SiLU's
+  s (1 + z (1 - s)) at z = -1.28), so what they are off by is absolute as well: 2^-21 max(1, |z|), times the factors beside
+  them, and as much as that of every term of a sum over deltaZ;
 A wrong part, tap, tail or index is orders above these (half the terms of a sum missing is an error of S)."""
 import math
 
@@ -254,16 +257,24 @@ def run_backward(kind, dy, z, act, x, w, want=("dx", "dw", "db"), pad=0):
     return {k: out[k].get() for k in want}
 
 
-def check_products(got, kind, names, dz, x, ws_, what):
-    """dx, dw and db of one pre-activation's gradient dz (fp64, unrounded)."""
+def delta_error(act, factor, z):
+    """What deltaZ = factor * act'(z) may be off by, in fp32 arithmetic (fp64 tensors): the derivative's and two roundings."""
+    if act == D.ACT_NONE:
+        return torch.zeros_like(factor)
+    return factor.abs() * 2.0 ** -21 * z.abs().clamp(min=1.0)
+
+
+ROUNDED = {"f32": 0.0, "bf16": 6 / math.sqrt(3) * 2.0 ** -8}      # deltaZ's rounding before its products
+
+
+def check_sums(got, kind, name_w, name_b, dz, edz, x, what):
+    """deltaW and deltaB of one pre-activation's gradient dz (fp64, unrounded), itself off by at most edz."""
     dtype = TYPES[kind][1]
-    extra = 6 / math.sqrt(3) * 2.0 ** -8 if kind == "bf16" else 2.0 ** -19
-    if names[1] in got:
-        close(got[names[1]], dz.t() @ x, product_tol(dz.t(), x.t(), dtype, extra), what + names[1])
-    if names[2] in got:
+    if name_w in got:
+        close(got[name_w], dz.t() @ x, product_tol(dz.t(), x.t(), dtype, ROUNDED[kind]) + edz.t() @ x.abs(), what + name_w)
+    if name_b in got:
         S = dz.square().sum(0, keepdim=True).sqrt()
-        close(got[names[2]], dz.sum(0, keepdim=True), S * (16 * math.sqrt(dz.shape[0] + 64) * 2.0 ** -23 + 2.0 ** -19), what + names[2])
-    return extra
+        close(got[name_b], dz.sum(0, keepdim=True), S * (16 * math.sqrt(dz.shape[0] + 64) * 2.0 ** -23) + edz.sum(0, keepdim=True), what + name_b)
 
 
 def check_backward(kind, n, ic, oc, act, want=("dx", "dw", "db"), pad=0, offset=0, seed=1):
@@ -272,10 +283,13 @@ def check_backward(kind, n, ic, oc, act, want=("dx", "dw", "db"), pad=0, offset=
     dy = matrix(n, oc, dtype, seed + 2, pad=pad, offset=offset)
     z = matrix(n, oc, dtype, seed + 3, pad=pad, offset=offset) if act != D.ACT_NONE else None
     got = run_backward(kind, dy, z, act, x, w, want, pad)
-    dz = dy.double() if z is None else dy.double() * slope64(act, z.double())
-    extra = check_products(got, kind, ("dx", "dw", "db"), dz, x.double(), None, "%s " % ((kind, n, ic, oc, act),))
+    dy64, z64, w64 = dy.double(), None if z is None else z.double(), w.double()
+    dz = dy64 if z is None else dy64 * slope64(act, z64)
+    edz = delta_error(act, dy64, z64)
+    what = "%s " % ((kind, n, ic, oc, act),)
+    check_sums(got, kind, "dw", "db", dz, edz, x.double(), what)
     if "dx" in want:
-        close(got["dx"], dz @ w.double(), product_tol(dz, w.double().t(), dtype, extra), "dx %s" % ((kind, n, ic, oc, act),))
+        close(got["dx"], dz @ w64, product_tol(dz, w64.t(), dtype, ROUNDED[kind]) + edz @ w64.abs(), what + "dx")
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -406,10 +420,13 @@ def check_gated_backward(kind, n, ic, oc, act=D.ACT_SILU, want=ALL_GATED, pad=0,
     dh64, g64, u64, x64 = dh.double(), g.double(), u.double(), x.double()
     dg, du = dh64 * u64 * slope64(act, g64), dh64 * act64(act, g64)
     what = "%s " % ((kind, n, ic, oc, act),)
-    extra = check_products(got, kind, ("dx", "dwg", "dbg"), dg, x64, None, what)
-    check_products(got, kind, ("dx", "dwu", "dbu"), du, x64, None, what)
+    edg = delta_error(act, dh64 * u64, g64)
+    edu = dh64.abs() * 2.0 ** -20 * g64.abs().clamp(min=1.0)          # act(g)'s own error
+    check_sums(got, kind, "dwg", "dbg", dg, edg, x64, what)
+    check_sums(got, kind, "dwu", "dbu", du, edu, x64, what)
     if "dx" in want:
-        tol = product_tol(torch.cat([dg, du], 1), torch.cat([wg.double(), wu.double()], 0).t(), dtype, extra)
+        tol = product_tol(torch.cat([dg, du], 1), torch.cat([wg.double(), wu.double()], 0).t(), dtype, ROUNDED[kind])
+        tol = tol + edg @ wg.double().abs() + edu @ wu.double().abs()
         close(got["dx"], dg @ wg.double() + du @ wu.double(), tol, what + "dx")
 
 
@@ -588,17 +605,19 @@ class Block:
         d = [t.double() for t in (self.x, self.wg, self.wu, self.wd, self.bd, self.dy)]
         x, wg, wu, wd, bd, dy = d
         close(y, h.double() @ wd.t() + bd + x, product_tol(h.double(), wd, self.dtype) + 2.0 ** -22 * (bd.abs() + x.abs() + 4), "y")
-        extra = 6 / math.sqrt(3) * 2.0 ** -8 if self.kind == "bf16" else 2.0 ** -19
+        extra = ROUNDED[self.kind]
         close(dh, dy @ wd, product_tol(dy, wd.t(), self.dtype), "dh")
         dg, du = dh.double() * u.double() * slope64(D.ACT_SILU, g.double()), dh.double() * act64(D.ACT_SILU, g.double())
-        close(dx, dg @ wg + du @ wu, product_tol(torch.cat([dg, du], 1), torch.cat([wg, wu]).t(), self.dtype, extra), "dx")
+        edg, edu = delta_error(D.ACT_SILU, dh.double() * u.double(), g.double()), dh.double().abs() * 2.0 ** -20 * g.double().abs().clamp(min=1.0)
+        tol = product_tol(torch.cat([dg, du], 1), torch.cat([wg, wu]).t(), self.dtype, extra) + edg @ wg.abs() + edu @ wu.abs()
+        close(dx, dg @ wg + du @ wu, tol, "dx")
         full = [dg.t() @ x, du.t() @ x, dy.t() @ h.double(), dy.sum(0)]
         total = math.sqrt(sum(float(t.square().sum()) for t in full))
         # the norm of the gradients as they were stored (rounded) is within their rounding of the exact ones'
         assert float(norm[0]) == pytest.approx(total, rel=2.0 ** -7 if self.kind == "bf16" else 1e-5)
         c = float(norm[1])
         assert c == pytest.approx(min(1.0, 1.0 / (float(norm[0]) + 1e-6)), rel=2.0 ** -22)
-        tols = [product_tol(dg.t(), x.t(), self.dtype, extra), product_tol(du.t(), x.t(), self.dtype, extra), product_tol(dy.t(), h.double().t(), self.dtype),
+        tols = [product_tol(dg.t(), x.t(), self.dtype, extra) + edg.t() @ x.abs(), product_tol(du.t(), x.t(), self.dtype, extra) + edu.t() @ x.abs(), product_tol(dy.t(), h.double().t(), self.dtype),
                 dy.square().sum(0).sqrt() * 16 * math.sqrt(self.n + 64) * 2.0 ** -23]
         for got, want, tol in zip((dwg, dwu, dwd, dbd), full, tols):
             # two roundings: the gradient's and the clipped one's
