@@ -31,7 +31,6 @@ int hip_status(hipError_t e, const char *what)
 inline long round8(long n) { return (n + 7) & ~7l; }
 inline size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 inline size_t size_of(int type) { return type == ALPHA_DENSE_F32 ? 4 : 2; }
-inline int parts_of(int type) { return type == ALPHA_DENSE_F32 ? 3 : 1; }
 
 // Takes blocks of the caller's workspace one after another; with no workspace it only counts.
 struct Scratch {
@@ -114,29 +113,27 @@ int check_distinct(const char *fn, const void *const *outputs, int n_out, const 
             return rc_;       \
     } while (0)
 
-// May the tile kernel's 128-bit loads read the tensor in place? Rows of whole 16-byte chunks, and nothing beyond a row's
-// end in its last chunk.
+// May the tile kernel read the tensor in place? fp32 always; bf16, whose 128-bit loads go straight to LDS, rows of whole 16-byte
+// chunks.
 bool in_place(int type, const void *p, int64_t stride, int cols)
 {
-    return type == ALPHA_DENSE_BF16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride & 7) == 0 && (cols & 7) == 0;
+    return type == ALPHA_DENSE_F32 || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride & 7) == 0 && (cols & 7) == 0);
 }
 
-// Room for a packed [rows, cols] tensor, whether the call will need it or not: the workspace does not depend on addresses.
-size_t packed_bytes(int type, long rows, long cols) { return (size_t)rows * round8(cols) * 2 * parts_of(type); }
+// Room for a packed [rows, cols] tensor, whether the call will need it or not: the workspace does not depend on addresses. fp32
+// needs it only for a pair of filters, whose row strides have to be one.
+size_t packed_bytes(int type, long rows, long cols, int pair = 0)
+{
+    return type == ALPHA_DENSE_F32 && !pair ? 0 : (size_t)rows * round8(cols) * size_of(type);
+}
 
 // One source of an operand of the tile kernel, packed if it has to be.
 int operand(const char *fn, hipStream_t s, int type, const void *p, int64_t stride, long rows, int cols, void *room, bool pack, DenseOperand &o, int which)
 {
-    o.plane = 0;
-    if (!pack) {
-        o.p[which] = static_cast<const __bf16 *>(p);
-        o.ld = stride;
-        return 0;
-    }
-    o.ld = round8(cols);
-    o.plane = rows * o.ld;
-    o.p[which] = static_cast<const __bf16 *>(room);
-    return hip_status(launch_dense_pack(s, type == ALPHA_DENSE_F32, p, stride, rows, cols, static_cast<__bf16 *>(room), o.ld, o.plane), fn);
+    o.p[which] = pack ? room : p;
+    o.ld = pack ? round8(cols) : stride;
+    if (!pack) return 0;
+    return hip_status(launch_dense_pack(s, type == ALPHA_DENSE_F32, p, stride, rows, cols, room, o.ld), fn);
 }
 
 int quads_aligned(int type, std::initializer_list<const void *> p, std::initializer_list<int64_t> strides)
@@ -162,15 +159,15 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
     ForwardRoom r{};
     if (dense_few_rows_preferred(type == ALPHA_DENSE_F32, gated, N, OC, IC)) return r;   // operands as they are, no pieces
     r.X = ws.take<void>(packed_bytes(type, N, IC));
-    for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC));
-    r.piece_bytes = dense_product_piece_bytes(N, OC, IC, parts_of(type), 1, gated);
+    for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
+    r.piece_bytes = dense_product_piece_bytes(N, OC, IC, type == ALPHA_DENSE_F32, 1, gated);
     r.pieces = ws.take<float>(r.piece_bytes);
     r.total = ws.at;
     return r;
 }
 
 struct BackwardRoom {
-    __bf16 *delta;
+    char *delta;
     void *X, *W[2];
     float *sums, *pieces;
     size_t piece_bytes, total;
@@ -180,14 +177,14 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
     Scratch ws(base);
     BackwardRoom r{};
     const int pair = gated ? 2 : 1;
-    r.delta = ws.take<__bf16>(packed_bytes(type, N, pair * round8(OC)));
+    r.delta = ws.take<char>((size_t)N * pair * round8(OC) * size_of(type));
     r.X = ws.take<void>(packed_bytes(type, N, IC));
-    for (int i = 0; i < pair; i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC));
+    for (int i = 0; i < pair; i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
     r.sums = ws.take<float>(dense_delta_sum_bytes(N, OC, gated));
-    const size_t for_x = dense_product_piece_bytes(N, IC, OC, parts_of(type), pair, 0);
+    const size_t for_x = dense_product_piece_bytes(N, IC, OC, type == ALPHA_DENSE_F32, pair, 0);
     // a gated pair's filter gradients are one stacked product, or one of them alone
-    const size_t for_w = std::max(dense_product_piece_bytes(OC, IC, N, parts_of(type), 1, 0),
-                                  gated ? dense_product_piece_bytes((int)round8(OC) + OC, IC, N, parts_of(type), 1, 0) : (size_t)0);
+    const size_t for_w = std::max(dense_product_piece_bytes(OC, IC, N, type == ALPHA_DENSE_F32, 1, 0),
+                                  gated ? dense_product_piece_bytes((int)round8(OC) + OC, IC, N, type == ALPHA_DENSE_F32, 1, 0) : (size_t)0);
     r.piece_bytes = std::max(for_x, for_w);
     r.pieces = ws.take<float>(r.piece_bytes);
     r.total = ws.at;
@@ -216,7 +213,6 @@ int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, i
     }
     const ForwardRoom room = forward_room(type, N, IC, OC, gated, workspace);
     DenseProduct p{};
-    p.parts = parts_of(type);
     p.sources = 1;
     p.gated = gated;
     p.M = N;
@@ -265,26 +261,23 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
     d.cols = OC;
     d.ld = round8(OC);
     d.ld2 = pair * d.ld;
-    d.plane = (long)N * d.ld2;
     d.dB = c.dB[0];
     d.dB2 = c.dB[1];
     d.sums = room.sums;
     DenseOperand delta{};
     if (!gated && act == ALPHA_DENSE_ACT_NONE && in_place(type, c.dY, c.ld_dY, OC)) {   // deltaZ is deltaY
-        delta.p[0] = static_cast<const __bf16 *>(c.dY);
+        delta.p[0] = c.dY;
         delta.ld = c.ld_dY;
     } else {
         if (products) d.dst = room.delta;
-        if (products && gated) d.dst2 = room.delta ? room.delta + d.ld : nullptr;
+        if (products && gated) d.dst2 = room.delta ? room.delta + d.ld * size_of(type) : nullptr;
         delta.p[0] = room.delta;
-        delta.p[1] = gated && room.delta ? room.delta + d.ld : nullptr;
+        delta.p[1] = gated && room.delta ? room.delta + d.ld * size_of(type) : nullptr;
         delta.ld = d.ld2;
-        delta.plane = d.plane;
     }
     if (d.dst || d.dB || d.dB2) TRY(hip_status(launch_dense_delta(s, d), fn));
 
     DenseProduct p{};
-    p.parts = parts_of(type);
     p.f32 = d.f32;
     p.pieces = room.pieces;
     p.piece_bytes = room.piece_bytes;

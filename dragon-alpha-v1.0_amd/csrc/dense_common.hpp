@@ -97,25 +97,6 @@ static __device__ __forceinline__ void quad_store(T *p, floatx4 v)
     *reinterpret_cast<typename Quad<T>::type *>(p) = q;
 }
 
-// ---- three-part split of an fp32 value -----------------------------------------------------------------------------
-// x = h + m + l exactly, each part a bf16 (8 significant bits, round to nearest, signs of the parts their own): 24 bits in
-// all. Where rounding up would leave bf16's range h is truncated; an infinity or NaN is h alone.
-static __device__ __forceinline__ void dense_split(float x, __bf16 &h, __bf16 &m, __bf16 &l)
-{
-    h = (__bf16)x;
-    const uint32_t bits = __float_as_uint(x);
-    if ((bits & 0x7fffffffu) >= 0x7f7f8000u) {
-        if ((bits & 0x7f800000u) == 0x7f800000u) {   // infinity or NaN
-            m = l = (__bf16)0.f;
-            return;
-        }
-        h = (__bf16)__uint_as_float(bits & 0xffff0000u);
-    }
-    const float r = x - (float)h;
-    m = (__bf16)r;
-    l = (__bf16)(r - (float)m);
-}
-
 // ---- the product's epilogue ----------------------------------------------------------------------------------------
 // Plain:  z = acc + bias[n];  Z = z;  Y = act(z) + R     (two stacked products, row2 > 0: rows m < rows1 to Y, m >= row2 to Y2)
 // Gated:  g = acc_g + bias[n], u = acc_u + bias2[n];  Z = g, Z2 = u;  Y = act(g) * u
@@ -129,28 +110,26 @@ struct DenseEpilogue {
     int vec;      // groups of four columns are aligned (bases and strides): vector accesses
 };
 
-// C[m, n] = sum over sources and k of A(m, k) B(n, k). An operand of the tile kernel is bf16; an fp32 tensor comes as
-// three of them (dense_split), `plane` elements apart.
+// C[m, n] = sum over sources and k of A(m, k) B(n, k). bf16 operands: rows of whole 16-byte chunks at 16-byte aligned
+// addresses, zeros after a row's last element; fp32: any.
 struct DenseOperand {
-    const __bf16 *p[2];   // up to two sources
+    const void *p[2];     // up to two sources
     long ld;              // element (row r, column c) at r * ld + c
-    long plane;
 };
 struct DenseProduct {
     DenseOperand A, B;
-    int parts;            // 1, or 3 (fp32: six of the nine products of parts)
     int sources;          // 2: the sum goes on over A.p[1], B.p[1]
     int gated;            // B.p[0], B.p[1] are the two filters of a gated pair
     int a_t, b_t;         // operand stored with k as its rows
     int M, N;             // N: of one filter where gated
     int K;
-    int f32;              // output type
+    int f32;
     DenseEpilogue ep;
     float *pieces;        // room for the pieces of cut reductions, `piece_bytes`
     size_t piece_bytes;
 };
-size_t dense_product_piece_bytes(int M, int N, int K, int parts, int sources, int gated);
-double dense_product_us(int M, int N, int K, int parts, int sources, int gated);   // the plan's estimate
+size_t dense_product_piece_bytes(int M, int N, int K, int f32, int sources, int gated);
+double dense_product_us(int M, int N, int K, int f32, int sources, int gated);   // the plan's estimate
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p);
 
 // Few rows, operands as they are (dense_few_rows.hip).
@@ -165,10 +144,10 @@ struct DenseFewRows {
 bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K);
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);
 
-// dst planes <- src[rows, cols]: fp32 in three parts, bf16 as it is; row stride ld (multiple of 8), columns cols .. ld zero.
-hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, __bf16 *dst, long ld, long plane);
+// dst <- src[rows, cols]; row stride ld (multiple of 8), columns cols .. ld zero.
+hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, void *dst, long ld);
 
-// deltaZ (or deltaG and deltaU) as packed planes and the column sums of the unrounded values.
+// deltaZ (or deltaG and deltaU) in the operands' type and the column sums of the unrounded values.
 struct DenseDelta {
     const void *dY, *Z, *U;
     long ldY, ldZ, ldU;
@@ -176,9 +155,9 @@ struct DenseDelta {
     float slope;
     long rows;
     int cols;
-    __bf16 *dst, *dst2;   // NULL: only the sums
+    void *dst, *dst2;     // NULL: only the sums
     long ld;              // columns written (cols, then zeros): a multiple of 8
-    long ld2, plane;      // row stride of dst, dst2
+    long ld2;             // row stride of dst, dst2
     void *dB, *dB2;       // NULL: no sums
     float *sums;          // dense_delta_sum_bytes of scratch
 };

@@ -170,9 +170,7 @@ bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K)
     const long groups = (long)((N + 15) / 16) * ((M + 63) / 64), rounds = (groups + cus - 1) / cus;
     const double turns = (double)K / (f32 ? 512 : 1024), turn = (f32 ? f32_turn : bf16_turn)[M > 32];
     const double us = 2.0 + rounds * (turns < 0.6 ? 0.6 : turns) * turn * (gated ? 1.4 : 1.0);
-    double other = dense_product_us(M, N, K, f32 ? 3 : 1, 1, gated);
-    if (f32) other += 6.0 + ((double)M + (double)N * (gated ? 2 : 1)) * K * 10 / 4e6;   // the split of both operands
-    return us < other;
+    return us < dense_product_us(M, N, K, f32, 1, gated);
 }
 
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a)

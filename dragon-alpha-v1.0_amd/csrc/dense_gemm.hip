@@ -40,10 +40,9 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
         for (int e = 0; e < 8; e++) {
             if (n + e >= a.N) break;
             if (v[e] != v[e])
-                v[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[0], a.B[1], (n + e) * b_row, b_k, a.planeB,
-                                     GATED ? 1 : a.combos / a.parts6, a.K);
+                v[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.B[0], a.B[1], (n + e) * b_row, b_k, GATED ? 1 : a.sources, a.K);
             if (GATED && u[e] != u[e])
-                u[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.planeA, a.B[1], a.B[1], (n + e) * b_row, b_k, a.planeB, 1, a.K);
+                u[e] = dense_element(a.A[0], a.A[0], m * a_row, a_k, a.B[1], a.B[1], (n + e) * b_row, b_k, 1, a.K);
         }
     }
     if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n, a.N);
@@ -63,17 +62,18 @@ size_t piece_bytes(const Plan &p) { return ((size_t)p.tiles_m * p.tiles_n - p.wh
 // Tile shape and cut: whole tiles for as many rounds as the device's workgroup slots go into, and the tiles that are left (or
 // all, where there are few) with their reduction cut so that they fill the device once more. The choice is the least of an
 // estimate of the device's time; its constants were measured on products of 256 x 256 x 256 to 8192 x 4096 x 4096: a
-// workgroup's step with the device nearly empty and full, 256 / 256 x 128 / 128: 0.57 / 0.34 / 0.36 and 0.70 / 0.48 / 0.59 us,
-// the last with two workgroups on a compute unit.
-Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t room)
+// workgroup's step with the device nearly empty and full, bf16 (256 / 256 x 128 / 128) 0.57 / 0.34 / 0.36 and 0.70 / 0.48 /
+// 0.59 us, the last with two workgroups on a compute unit; fp32 (256 x 128 / 128) 1.6 / 0.9 and 1.9 / 1.1.
+Plan make_plan(int M, int N, int K, int f32, int sources, int gated, size_t room)
 {
-    static constexpr double empty[DENSE_TILES] = {0.57, 0.34, 0.36}, full[DENSE_TILES] = {0.70, 0.48, 0.59}, fixed[DENSE_TILES] = {6.5, 5.0, 3.0};
+    static constexpr double empty[2][DENSE_TILES] = {{0.57, 0.34, 0.36}, {0, 1.6, 0.9}}, full[2][DENSE_TILES] = {{0.70, 0.48, 0.59}, {0, 1.9, 1.1}};
+    static constexpr double fixed[DENSE_TILES] = {6.5, 5.0, 3.0};
     const int cus = std::max(1, device_cu_count());
-    const int nk = std::max(1, (K + 31) / 32), combos = (parts == 3 ? 6 : 1) * sources, steps = nk * combos;
+    const int nk = std::max(1, (K + 31) / 32), steps = nk * sources;
     const double bytes_per_us = 4.2e6, outputs = (double)M * N * (gated ? 2 : 1);
     Plan best{};
     best.us = 1e30;
-    for (int t = 0; t < DENSE_TILES; t++) {
+    for (int t = f32 ? DENSE_TILE_256_128 : DENSE_TILE_256; t < DENSE_TILES; t++) {
         const int bm = DENSE_TILE_M[t], bn = DENSE_TILE_N[t];
         Plan p{};
         p.tile = (DenseTile)t;
@@ -81,29 +81,30 @@ Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t ro
         p.tiles_n = (N * (gated ? 2 : 1) + bn - 1) / bn;
         p.steps = steps;
         const long tiles = (long)p.tiles_m * p.tiles_n;
+        const double e = empty[f32 ? 1 : 0][t], f = full[f32 ? 1 : 0][t];
+        const bool shared = t == DENSE_TILE_128 && !f32;     // two workgroups on a compute unit
         // time of `groups` workgroups of `per` steps each
         auto rounds_us = [&](long groups, int per) {
-            const bool pairs = t == DENSE_TILE_128 && groups > cus;
+            const bool pairs = shared && groups > cus;
             const long slots = pairs ? 2l * cus : cus, rounds = (groups + slots - 1) / slots;
             const double filled = std::min(1.0, (double)groups / slots);
-            return rounds * (per * (t == DENSE_TILE_128 ? (pairs ? full[t] : empty[t]) : empty[t] + (full[t] - empty[t]) * filled) + fixed[t]);
+            return rounds * (per * (shared ? (pairs ? f : e) : e + (f - e) * filled) + fixed[t]);
         };
         auto consider = [&](long whole, int split) {
-            // whole k steps: a piece holds all parts of its products, so none leaves fp32's range that the sum would not
-            // (and an even number of steps: the kernel's loop does two at a time)
+            // (an even number of steps: the kernels' loops do two at a time)
             p.whole = (int)whole;
             p.split = split;
-            p.per = (nk + 2 * split - 1) / (2 * split) * 2 * combos;
+            p.per = (nk + 2 * split - 1) / (2 * split) * 2 * sources;
             const long left = tiles - whole;
-            p.us = 3.5 + outputs * (parts == 3 ? 4 : 2) / bytes_per_us + (whole > 0 ? rounds_us(whole, steps) : 0.0);
+            p.us = 3.5 + outputs * (f32 ? 4 : 2) / bytes_per_us + (whole > 0 ? rounds_us(whole, steps) : 0.0);
             if (left > 0) {
-                if (split < 2 || p.per < 8 || (steps + p.per - 1) / p.per != split || piece_bytes(p) > room) return;   // (every piece has a step)
+                if (split < 2 || p.per < (f32 ? 2 : 8) || (steps + p.per - 1) / p.per != split || piece_bytes(p) > room) return;   // (every piece has a step)
                 p.us += rounds_us(left * split, p.per) + 4.5 + piece_bytes(p) * 2.0 / bytes_per_us;
             }
             if (p.us < best.us) best = p;
         };
         consider(tiles, 1);
-        const long slots = t == DENSE_TILE_128 ? 2l * cus : cus, starts[2] = {0, tiles / slots * slots};
+        const long slots = shared ? 2l * cus : cus, starts[2] = {0, tiles / slots * slots};
         for (int i = 0; i < 2; i++) {
             if ((i == 1 && starts[1] == 0) || starts[i] == tiles || tiles - starts[i] > slots) continue;
             for (int split = 2; split <= 64; split += split < 8 ? 1 : split < 16 ? 2 : 8) consider(starts[i], split);
@@ -114,18 +115,18 @@ Plan make_plan(int M, int N, int K, int parts, int sources, int gated, size_t ro
 
 }  // namespace
 
-size_t dense_product_piece_bytes(int M, int N, int K, int parts, int sources, int gated)
+size_t dense_product_piece_bytes(int M, int N, int K, int f32, int sources, int gated)
 {
     // as many pieces as the plan without a limit takes
-    return piece_bytes(make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60));
+    return piece_bytes(make_plan(M, N, K, f32, sources, gated, (size_t)1 << 60));
 }
 
-double dense_product_us(int M, int N, int K, int parts, int sources, int gated) { return make_plan(M, N, K, parts, sources, gated, (size_t)1 << 60).us; }
+double dense_product_us(int M, int N, int K, int f32, int sources, int gated) { return make_plan(M, N, K, f32, sources, gated, (size_t)1 << 60).us; }
 
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
 {
     if (p.M <= 0 || p.N <= 0) return hipSuccess;
-    const Plan plan = make_plan(p.M, p.N, p.K, p.parts, p.sources, p.gated, p.pieces ? p.piece_bytes : 0);
+    const Plan plan = make_plan(p.M, p.N, p.K, p.f32, p.sources, p.gated, p.pieces ? p.piece_bytes : 0);
     DenseTileArgs a{};
     for (int i = 0; i < 2; i++) {
         a.A[i] = p.A.p[i];
@@ -133,13 +134,10 @@ hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
     }
     a.ldA = p.A.ld;
     a.ldB = p.B.ld;
-    a.planeA = p.A.plane;
-    a.planeB = p.B.plane;
     a.M = p.M;
     a.N = p.N;
     a.K = p.K;
-    a.parts6 = p.parts == 3 ? 6 : 1;
-    a.combos = a.parts6 * p.sources;
+    a.sources = p.sources;
     a.steps = plan.steps;
     a.whole = plan.whole;
     a.split = plan.split;

@@ -15,43 +15,9 @@
 // bytes: stored from the registers as they are, 4096 x 4096 of bf16 took 17 us to write, this way 10.
 // Gated: of every 64 tile columns 32 are of one filter and 32, the same ones, of the other.
 #pragma once
-#include "dense_finish.hpp"
-
-#include <type_traits>
+#include "dense_tile.hpp"
 
 namespace alpha {
-
-typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
-typedef short shortx4 __attribute__((ext_vector_type(4)));
-
-struct DenseTileArgs {
-    const __bf16 *A[2], *B[2];
-    long ldA, ldB, planeA, planeB;
-    int M, N, K;
-    int combos;        // products per 32 k: parts (1 or 6) x sources
-    int parts6;        // 6 for the three-part split, else 1
-    int steps;         // combos for every 32 k
-    int tiles_m, tiles_n;
-    int whole;         // the first `whole` tiles are a workgroup's whole work; the others' reductions are cut
-    int split, per;    // into `split` runs of `per` steps (an even number)
-    DenseEpilogue ep;
-    float *pieces;     // [split][tiles - whole][BM][BN], as the tile kernel has them
-};
-
-// The XCD-aware order of tiles. Workgroups go round the eight XCDs, so every eighth one shares an L2: an XCD gets a contiguous
-// run of `count` places.
-static __device__ __forceinline__ int xcd_place(int id, int count)
-{
-    const int each = count / 8, more = count % 8, xcd = id & 7;
-    return xcd * each + (xcd < more ? xcd : more) + (id >> 3);
-}
-// Tile number -> tile row and column: panels of 8 tile rows, so that a run of tiles reuses both operands out of the L2.
-static __device__ __forceinline__ void tile_at(int tile, int tiles_m, int tiles_n, int &tm, int &tn)
-{
-    const int panel = tile / (8 * tiles_n), first = panel * 8, deep = tiles_m - first < 8 ? tiles_m - first : 8, in = tile - panel * 8 * tiles_n;
-    tm = first + in % deep;
-    tn = in / deep;
-}
 
 static __device__ __forceinline__ void load_to_lds(unsigned lds, unsigned voffset, uintx4 rsrc)
 {
@@ -66,56 +32,7 @@ static __device__ __forceinline__ uintx4 make_rsrc(const void *p, unsigned bytes
     return uintx4{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 
-// which parts the c-th of the six products multiplies: (l,h) (h,l) (m,m) (m,h) (h,m) (h,h), small ones first
-static __device__ __forceinline__ int combo_part_a(int c) { return (0x052 >> (2 * c)) & 3; }
-static __device__ __forceinline__ int combo_part_b(int c) { return (0x118 >> (2 * c)) & 3; }
-
-// One element of C once more in plain fp32, from the parts: taken where the sum of the parts' products is NaN, which it
-// also is where one operand is infinite and a part of the other zero. Ends at the first NaN.
-static __device__ __attribute__((noinline)) float dense_element(const __bf16 *A0, const __bf16 *A1, long a_row, long a_k, long planeA,
-                                                                const __bf16 *B0, const __bf16 *B1, long b_row, long b_k, long planeB,
-                                                                int sources, int K)
-{
-    float acc = 0.f;
-    for (int s = 0; s < sources; s++) {
-        const __bf16 *a = (s ? A1 : A0) + a_row, *b = (s ? B1 : B0) + b_row;
-        for (int k = 0; k < K; k++, a += a_k, b += b_k) {
-            const float x = (float)a[0] + (float)a[planeA] + (float)a[2 * planeA];
-            const float y = (float)b[0] + (float)b[planeB] + (float)b[2 * planeB];
-            acc = fmaf(x, y, acc);
-            if (acc != acc) return acc;
-        }
-    }
-    return acc;
-}
-
-// f(0), f(1), .. f(N - 1) with constants: unrolled whatever its size
-template <int N, int I = 0, typename F>
-static __device__ __forceinline__ void for_each(F &&f)
-{
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        for_each<N, I + 1>(f);
-    }
-}
-
-// Between LDS accesses of one wavefront's lanes: LDS serves a wavefront in order, the compiler must keep that order.
-static __device__ __forceinline__ void wave_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Which 16-byte chunk of a T tile's k row a chunk is kept at: number ^ this. The 32 lanes that one cycle of a transposing
-// read serves touch eight k rows (0 .. 3 and 8 .. 11), whose 32-byte pieces so lie in eight different parts of the 256 bytes
-// that a cycle delivers.
-static __device__ __forceinline__ int t_permutation(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
-// The same for a straight tile, by g = row / 4. The 16 lanes that a cycle of a 128-bit read serves are rows 0-3 and 12-15
-// of a fragment in one chunk and rows 4-11 in the chunk beside it (or the other way round); four rows are 256 bytes, so the
-// four groups of rows must come to four different chunks: 0, 3, 2, 1 for g = 0 .. 3. Counted: no conflicts.
-static __device__ __forceinline__ int s_permutation(int g) { return (g & 1) | ((g ^ (g >> 1)) & 1) << 1; }
-
-template <typename T, bool AT, bool BT, bool GATED, int BM, int BN, int WM, int WN, int STAGES>
+template <bool AT, bool BT, bool GATED, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const DenseTileArgs a)
 {
     constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
@@ -175,12 +92,13 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     const int t0 = piece * a.per;
     int left = a.steps - t0;
     if (cut && left > a.per) left = a.per;
-    int combo = t0 % a.combos;                         // of the next step to load
-    int krem = a.K - t0 / a.combos * 32;               // k from its first on; <= 0: nothing, zeros
+    int source = t0 % a.sources;                       // of the next step to load
+    int krem = a.K - t0 / a.sources * 32;              // k from its first on; <= 0: nothing, zeros
     const long stepA = AT ? 32 * a.ldA : 32, stepB = BT ? 32 * a.ldB : 32;
     const long atA = AT ? (long)m0 : (long)m0 * a.ldA, atB = BT ? (long)n0 : (long)n0 * a.ldB;
-    const __bf16 *pA = a.A[0] + atA + t0 / a.combos * stepA, *pB = a.B[0] + atB + t0 / a.combos * stepB;   // first source, first part
-    const long toA1 = a.A[1] - a.A[0], toB1 = a.B[1] - a.B[0];
+    const __bf16 *const A0 = static_cast<const __bf16 *>(a.A[0]), *const B0 = static_cast<const __bf16 *>(a.B[0]);
+    const __bf16 *pA = A0 + atA + t0 / a.sources * stepA, *pB = B0 + atB + t0 / a.sources * stepB;   // in the first source
+    const long toA1 = static_cast<const __bf16 *>(a.A[1]) - A0, toB1 = static_cast<const __bf16 *>(a.B[1]) - B0;
     // bytes from a tile's first element to its end: straight, its rows' last chunk; T, of one k row
     const int spanN = GATED ? BN / 2 : BN;
     const unsigned endA = AT ? (unsigned)((a.M - m0 + 7) & ~7) * 2 : (unsigned)(((long)((a.M - m0 < BM ? a.M - m0 : BM) - 1) * a.ldA + 32) * 2);
@@ -196,17 +114,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
         if (part == 0) {
             qA = pA;
             qB = pB;
-            if (a.combos > 1) {   // uniform
-                const bool second = combo >= a.parts6;
-                const int c = second ? combo - a.parts6 : combo;
-                if (second) {
-                    qA += toA1;
-                    qB += toB1;
-                }
-                if (a.parts6 == 6) {
-                    qA += combo_part_a(c) * a.planeA;
-                    qB += combo_part_b(c) * a.planeB;
-                }
+            if (source) {   // uniform
+                qA += toA1;
+                qB += toB1;
             }
             if (GATED && (wave & 2)) qB += toB1;
         } else if (part == 1) {
@@ -219,8 +129,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
             inB = BT || kchunkB < krem;
         } else {
             lds = __builtin_amdgcn_readfirstlane(lds0 + stage + wave * 1024);
-            if (++combo == a.combos) {
-                combo = 0;
+            if (++source == a.sources) {
+                source = 0;
                 krem -= 32;
                 pA += stepA;
                 pB += stepB;
@@ -233,7 +143,6 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     };
 
     // ---- where the fragments are read ----
-    typedef __attribute__((address_space(3))) char lds_char;
     unsigned rdA[AT ? MF : 1], rdB[BT ? NF : 1];                 // (a T fragment's piece is permuted by the lane: an address each)
     const int tk = q * 8 + (l16 >> 2), t16 = (l16 & 3) >> 1;     // T: the lane's k row and 16-byte half of a piece
     const int chunk = (q ^ s_permutation(l16 >> 2)) * 16;
@@ -320,69 +229,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // every load into LDS has landed, every read of it is done
 
-    // ---- out: two fragment rows (32 rows of C) at a time through the wavefront's part of LDS ----
-    constexpr int ROW = 68;                              // floats from row to row: 16 bytes past a multiple of the banks
-    constexpr int LANES = GATED ? 4 : 8;                 // lanes of a row, eight columns each (gated: eight of each filter)
-    constexpr int AT_ONCE = 64 / LANES, TURNS = 32 / AT_ONCE;
-    static_assert(TN == 64, "a wavefront's rows are 64 columns");
-    static_assert(WM * WN * 32 * ROW * 4 <= (int)RING, "the ring holds the parts");
-    float *const part = reinterpret_cast<float *>(smem) + wave * (32 * ROW);
-    const int at = (lane % LANES) * 8, n = n0 + wn * (GATED ? 32 : 64) + at;
-    unsigned again = 0;   // fp32: runs with a NaN among them, computed once more below
-#pragma unroll
-    for (int i = 0; i < MF; i += 2) {
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[i + h][j];
-        wave_fence();
-#pragma unroll 1
-        for (int y = 0; y < 32; y += AT_ONCE) {
-            const int row = y + lane / LANES;
-            const long m = m0 + wm * TM + i * 16 + row;
-            float v[8], u[8];
-            run_load(part + row * ROW + at, v);
-            if constexpr (GATED) run_load(part + row * ROW + 32 + at, u);
-            if (m >= a.M || n >= a.N) continue;
-            if (cut) {
-                float *dst = a.pieces + (((long)piece * cut_tiles + (tile - a.whole)) * BM + (wm * TM + i * 16 + row)) * BN + wn * TN + at;
-                run_store(dst, v);
-                if constexpr (GATED) run_store(dst + 32, u);
-            } else {
-                if constexpr (__is_same(T, float)) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
-                    if (sum != sum) {   // (also where infinities of both signs meet: no harm)
-                        again |= 1u << (i / 2 * TURNS + y / AT_ONCE);
-                        continue;
-                    }
-                }
-                if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n, a.N);
-                else dense_finish<T>(a.ep, v, m, n, a.N);
-            }
-        }
-        wave_fence();
-    }
-    if constexpr (__is_same(T, float)) {
-        static_assert(MF / 2 * TURNS <= 32, "one bit per run");
-        while (again) {
-            const int bit = __ffs(again) - 1;
-            again &= again - 1;
-            const long m = m0 + wm * TM + bit / TURNS * 32 + bit % TURNS * AT_ONCE + lane / LANES;
-            for (int e = 0; e < 8 && n + e < a.N; e++) {
-                float v[1], u[1] = {0.f};
-                v[0] = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.planeA, a.B[0], a.B[1], BT ? n + e : (n + e) * a.ldB,
-                                     BT ? a.ldB : 1, a.planeB, GATED ? 1 : a.combos / a.parts6, a.K);
-                if constexpr (GATED) {
-                    u[0] = dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.planeA, a.B[1], a.B[1], (n + e) * a.ldB, 1, a.planeB, 1, a.K);
-                    dense_finish_gated<T>(a.ep, v, u, m, n + e, a.N);
-                } else {
-                    dense_finish<T>(a.ep, v, m, n + e, a.N);
-                }
-            }
-        }
-    }
+    tile_out<__bf16, AT, BT, GATED, BM, BN, WM, WN, RING>(a, acc, smem, lane, wave, wm, wn, m0, n0, cut, piece, tile - a.whole, cut_tiles);
 }
 
 }  // namespace alpha

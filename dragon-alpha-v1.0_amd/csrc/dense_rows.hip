@@ -1,6 +1,5 @@
-// The passes around a dense product, each bound by memory: operands made ready for the tile kernel (three-part split of
-// fp32, rows of bf16 that the 128-bit loads cannot take copied to ones they can), and deltaZ = deltaY * act'(Z) with its
-// column sums.
+// The passes around a dense product, each bound by memory: rows of bf16 that the tile kernel's 128-bit loads cannot take copied
+// to ones they can, and deltaZ = deltaY * act'(Z) with its column sums.
 #include "dense_common.hpp"
 
 #include <algorithm>
@@ -31,59 +30,59 @@ __device__ __forceinline__ void load8(const T *row, int c, int cols, float (&v)[
     for (int e = 0; e < 8; e++) v[e] = c + e < cols ? dense_load(row + c + e) : 0.f;
 }
 
+// eight elements at an address aligned to 16 bytes
 template <typename T>
-__device__ __forceinline__ void store_parts(__bf16 *dst, long plane, const float (&v)[8])
+__device__ __forceinline__ void store8(T *dst, const float (&v)[8])
 {
-    bf16x8 h, m, l;
-    if constexpr (__is_same(T, float)) {
+    if constexpr (sizeof(T) == 2) {
+        bf16x8 t;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            __bf16 x, y, z;
-            dense_split(v[e], x, y, z);
-            h[e] = x, m[e] = y, l[e] = z;
-        }
-        *reinterpret_cast<bf16x8 *>(dst + plane) = m;
-        *reinterpret_cast<bf16x8 *>(dst + 2 * plane) = l;
+        for (int e = 0; e < 8; e++) t[e] = (__bf16)v[e];
+        *reinterpret_cast<bf16x8 *>(dst) = t;
     } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) h[e] = (__bf16)v[e];
+        quad_store(dst, floatx4{v[0], v[1], v[2], v[3]});
+        quad_store(dst + 4, floatx4{v[4], v[5], v[6], v[7]});
     }
-    *reinterpret_cast<bf16x8 *>(dst) = h;
 }
 
 }  // namespace
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void dense_pack_kernel(const T *__restrict__ src, long src_ld, long total, int cols, __bf16 *__restrict__ dst,
-                                                         long ld, long plane, FastDiv d_chunks)
+__global__ __launch_bounds__(256) void dense_pack_kernel(const T *__restrict__ src, long src_ld, long total, int cols, T *__restrict__ dst,
+                                                         long ld, FastDiv d_chunks)
 {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long row = fdiv((uint32_t)i, d_chunks);
         const int c = (int)(i - row * d_chunks.d) * 8;
         float v[8];
         load8<T, VEC>(src + row * src_ld, c, cols, v);
-        store_parts<T>(dst + row * ld + c, plane, v);
+        store8(dst + row * ld + c, v);
     }
 }
 
-hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, __bf16 *dst, long ld, long plane)
+namespace {
+
+template <typename T>
+hipError_t launch_pack(hipStream_t s, const void *src, long src_ld, long total, int cols, void *dst, long ld)
 {
-    const long chunks = ld / 8, total = rows * chunks;
+    const dim3 grid((unsigned)std::min<long>((total + 255) / 256, 16384));
+    const FastDiv d = make_fastdiv((uint32_t)(ld / 8));
+    const T *p = static_cast<const T *>(src);
+    if ((reinterpret_cast<uintptr_t>(src) & (4 * sizeof(T) - 1)) == 0 && (src_ld & 3) == 0)
+        hipLaunchKernelGGL((dense_pack_kernel<T, true>), grid, dim3(256), 0, s, p, src_ld, total, cols, static_cast<T *>(dst), ld, d);
+    else
+        hipLaunchKernelGGL((dense_pack_kernel<T, false>), grid, dim3(256), 0, s, p, src_ld, total, cols, static_cast<T *>(dst), ld, d);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, void *dst, long ld)
+{
+    const long total = rows * (ld / 8);
     if (total <= 0) return hipSuccess;
     if (total >= (1l << 31)) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)std::min<long>((total + 255) / 256, 16384));
-    const FastDiv d = make_fastdiv((uint32_t)chunks);
-    const bool vec = (reinterpret_cast<uintptr_t>(src) & (f32 ? 15 : 7)) == 0 && (src_ld & 3) == 0;
-    if (f32) {
-        const float *p = static_cast<const float *>(src);
-        if (vec) hipLaunchKernelGGL((dense_pack_kernel<float, true>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
-        else hipLaunchKernelGGL((dense_pack_kernel<float, false>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
-    } else {
-        const __bf16 *p = static_cast<const __bf16 *>(src);
-        if (vec) hipLaunchKernelGGL((dense_pack_kernel<__bf16, true>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
-        else hipLaunchKernelGGL((dense_pack_kernel<__bf16, false>), grid, dim3(256), 0, s, p, src_ld, total, cols, dst, ld, plane, d);
-    }
-    return hipGetLastError();
+    return f32 ? launch_pack<float>(s, src, src_ld, total, cols, dst, ld) : launch_pack<__bf16>(s, src, src_ld, total, cols, dst, ld);
 }
 
 // A workgroup takes 256 columns (32 lanes of 8) of a run of rows, eight rows at a time; its column sums go to sums[run].
@@ -115,9 +114,9 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, lo
                 sum[e] += dy[e];
                 if constexpr (GATED) sum2[e] += out2[e];
             }
-            if (d.dst) store_parts<T>(d.dst + r * d.ld2 + c, d.plane, dy);
+            if (d.dst) store8(static_cast<T *>(d.dst) + r * d.ld2 + c, dy);
             if constexpr (GATED)
-                if (d.dst2) store_parts<T>(d.dst2 + r * d.ld2 + c, d.plane, out2);
+                if (d.dst2) store8(static_cast<T *>(d.dst2) + r * d.ld2 + c, out2);
         }
     }
     if (!d.sums) return;
