@@ -292,11 +292,13 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
         p.ep.Y = c.dX;
         p.ep.ldY = c.ld_dX;
         p.ep.vec = quads_aligned(type, {c.dX}, {c.ld_dX});
+        const bool small = dense_small_preferred(p.f32, p.M, p.N, p.K, p.sources);
         if (OC > 0) {
-            const bool pack = !in_place(type, c.W[0], c.ldW[0], IC) || (gated && (!in_place(type, c.W[1], c.ldW[1], IC) || c.ldW[0] != c.ldW[1]));
+            const bool strides = gated && c.ldW[0] != c.ldW[1];
+            const bool pack = strides || (!small && (!in_place(type, c.W[0], c.ldW[0], IC) || (gated && !in_place(type, c.W[1], c.ldW[1], IC))));
             for (int i = 0; i < pair; i++) TRY(operand(fn, s, type, c.W[i], c.ldW[i], OC, IC, room.W[i], pack, p.B, i));
         }
-        TRY(hip_status(launch_dense_product(s, p), fn));
+        TRY(hip_status(small ? launch_dense_small(s, p) : launch_dense_product(s, p), fn));
     }
     if (want_w) {   // deltaW[oc, ic] = sum over n; both filters' as one product over the pair's columns
         p.A = delta;
@@ -320,8 +322,9 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
             p.ep.ldY2 = c.ld_dW[1];
             p.ep.vec = p.ep.vec && quads_aligned(type, {c.dW[1]}, {c.ld_dW[1]});
         }
-        if (N > 0) TRY(operand(fn, s, type, c.X, c.ldX, N, IC, room.X, !in_place(type, c.X, c.ldX, IC), p.B, 0));
-        TRY(hip_status(launch_dense_product(s, p), fn));
+        const bool small = dense_small_preferred(p.f32, p.M, p.N, p.K, 1);
+        if (N > 0) TRY(operand(fn, s, type, c.X, c.ldX, N, IC, room.X, !small && !in_place(type, c.X, c.ldX, IC), p.B, 0));
+        TRY(hip_status(small ? launch_dense_small(s, p) : launch_dense_product(s, p), fn));
     }
     return 0;
 }

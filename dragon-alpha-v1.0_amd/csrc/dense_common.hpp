@@ -97,6 +97,25 @@ static __device__ __forceinline__ void quad_store(T *p, floatx4 v)
     *reinterpret_cast<typename Quad<T>::type *>(p) = q;
 }
 
+// COLS consecutive elements of a row from column c on, whatever their alignment. At the row's end (`cols` >= COLS) the last
+// COLS are loaded instead, without a branch, and moved to their places by at_edge: zeros from `cols` on.
+template <int COLS, typename T>
+static __device__ __forceinline__ void load_columns(const T *row, int c, int cols, T (&v)[COLS])
+{
+    __builtin_memcpy(v, row + (c < cols - COLS ? c : cols - COLS), COLS * sizeof(T));
+}
+template <int COLS, typename T>
+static __device__ __forceinline__ void at_edge(int c, int cols, T (&v)[COLS])
+{
+    const int by = c - (cols - COLS);
+#pragma unroll
+    for (int i = 0; i < COLS; i++) {
+        const bool move = by > i;
+#pragma unroll
+        for (int e = 0; e < COLS; e++) v[e] = move ? (e + 1 < COLS ? v[e + 1] : (T)0.f) : v[e];
+    }
+}
+
 // ---- the product's epilogue ----------------------------------------------------------------------------------------
 // Plain:  z = acc + bias[n];  Z = z;  Y = act(z) + R     (two stacked products, row2 > 0: rows m < rows1 to Y, m >= row2 to Y2)
 // Gated:  g = acc_g + bias[n], u = acc_u + bias2[n];  Z = g, Z2 = u;  Y = act(g) * u
@@ -143,6 +162,10 @@ struct DenseFewRows {
 
 bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K);
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);
+
+// Small products of a backward (B with k as its rows), operands as they are, no pieces (dense_small.hip).
+bool dense_small_preferred(int f32, int M, int N, int K, int sources);
+hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p);
 
 // dst <- src[rows, cols]; row stride ld (multiple of 8), columns cols .. ld zero.
 hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, void *dst, long ld);

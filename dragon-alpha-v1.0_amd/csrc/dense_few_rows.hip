@@ -9,7 +9,7 @@
 // At most four rows of X: four columns a workgroup instead of 16, the MFMA's 16 rows and columns being four pieces of the
 // reduction times four (only the products of equal pieces are read out): four times as many workgroups, each with a
 // quarter of the reduction's length in turns (1 x 8192 x 1024: 11.4 -> 6.5 us).
-// Rows may begin at any element; only where K is no multiple of 16 bytes is the last piece read element by element.
+// Rows may begin at any element and K may be any number.
 #include "dense_finish.hpp"
 
 namespace alpha {
@@ -35,16 +35,18 @@ template <typename T>
 __device__ __forceinline__ typename FewVec<T>::type few_load_tail(const T *row, int k, int K)
 {
     constexpr int V = 16 / sizeof(T);
-    typename FewVec<T>::type v;
-    if (K % V == 0) {   // uniform: all of it or nothing, without a branch (k = 0 exists)
-        v = few_load(row, k < K ? k : 0);
-#pragma unroll
-        for (int e = 0; e < V; e++) v[e] = k < K ? v[e] : (T)0.f;
+    T v[V];
+    if (K >= V) {   // uniform
+        load_columns<V>(row, k, K, v);
+        at_edge<V>(k, K, v);
     } else {
 #pragma unroll
         for (int e = 0; e < V; e++) v[e] = k + e < K ? row[k + e] : (T)0.f;
     }
-    return v;
+    typename FewVec<T>::type out;
+#pragma unroll
+    for (int e = 0; e < V; e++) out[e] = v[e];
+    return out;
 }
 
 __device__ __forceinline__ floatx4 few_multiply(bf16x8 w, bf16x8 x, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
@@ -138,8 +140,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
                 v[0] += reinterpret_cast<const float *>(&part[s][b][at])[col & 3];
                 if constexpr (GATED) u[0] += reinterpret_cast<const float *>(&part[s][(GATED ? MB : 0) + b][at])[col & 3];
             }
-        if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n0 + col, a.N);
-        else dense_finish<T>(a.ep, v, m, n0 + col, a.N);
+        if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n0 + col);
+        else dense_finish<T, 1, true>(a.ep, v, m, n0 + col);
     }
 }
 

@@ -4,10 +4,12 @@
 
 namespace alpha {
 
-// R consecutive elements of a row, aligned to groups of four.
+// R consecutive elements of a row, aligned to groups of four, or one element.
 template <int R, typename T>
 static __device__ __forceinline__ void run_load(const T *p, float (&v)[R])
 {
+    if constexpr (R == 1) v[0] = dense_load(p);
+    else
 #pragma unroll
     for (int i = 0; i < R; i += 4) {
         const floatx4 q = quad_load(p + i);
@@ -18,7 +20,9 @@ static __device__ __forceinline__ void run_load(const T *p, float (&v)[R])
 template <int R, typename T>
 static __device__ __forceinline__ void run_store(T *p, const float (&v)[R])
 {
-    if constexpr (R == 8 && sizeof(T) == 2) {   // one 128-bit store (the hardware takes 8-byte alignment)
+    if constexpr (R == 1) {
+        dense_store(p, v[0]);
+    } else if constexpr (R == 8 && sizeof(T) == 2) {   // one 128-bit store (the hardware takes 8-byte alignment)
         bf16x8 q;
 #pragma unroll
         for (int e = 0; e < 8; e++) q[e] = (T)v[e];
@@ -52,97 +56,56 @@ static __device__ __forceinline__ void run_act(int act, float (&v)[R], float k)
     }
 }
 
-// The epilogues of R consecutive columns n .. n+R-1 of row m (fewer at the right edge).
-template <typename T, int R>
-static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n, int N)
+// The epilogues of R consecutive columns n .. n+R-1 of row m, R a multiple of four and aligned to it, or one element. FULL: all
+// of the epilogue; else only the store (the products of a backward).
+template <typename T, int R, bool FULL>
+static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n)
 {
-    const bool second = ep.row2 > 0 && m >= ep.row2;
-    if (ep.row2 > 0 && !second && m >= ep.rows1) return;   // a row between two stacked products
+    const bool second = !FULL && ep.row2 > 0 && m >= ep.row2;
+    if (!FULL && ep.row2 > 0 && !second && m >= ep.rows1) return;   // a row between two stacked products
     T *Y = static_cast<T *>(second ? ep.Y2 : ep.Y) + (second ? (m - ep.row2) * ep.ldY2 : m * ep.ldY) + n;
-    const T *bias = static_cast<const T *>(ep.bias), *res = static_cast<const T *>(ep.R);
-    T *Z = static_cast<T *>(ep.Z);
-    const bool whole = R % 4 == 0 && ep.vec && n + R <= N;
-    float t[R];
-    if (bias) {
-        if constexpr (R % 4 == 0)
-            if (whole) run_load(bias + n, t);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(bias + n + e) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] += t[e];
-    }
-    if (Z) {
-        if constexpr (R % 4 == 0)
-            if (whole) run_store(Z + m * ep.ldZ + n, v);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < R; e++)
-                if (n + e < N) dense_store(Z + m * ep.ldZ + n + e, v[e]);
-        }
-    }
-    run_act<T>(ep.act, v, ep.slope);
-    if (res) {
-        if constexpr (R % 4 == 0)
-            if (whole) run_load(res + m * ep.ldR + n, t);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(res + m * ep.ldR + n + e) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < R; e++) v[e] += t[e];
-    }
-    if constexpr (R % 4 == 0)
-        if (whole) run_store(Y, v);
-    if (!whole) {
-#pragma unroll
-        for (int e = 0; e < R; e++)
-            if (n + e < N) dense_store(Y + e, v[e]);
-    }
-}
-
-template <typename T, int R>
-static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &ep, float (&g)[R], float (&u)[R], long m, int n, int N)
-{
-    T *Y = static_cast<T *>(ep.Y) + m * ep.ldY + n;
-    const bool whole = R % 4 == 0 && ep.vec && n + R <= N;
-#pragma unroll
-    for (int which = 0; which < 2; which++) {
-        float(&v)[R] = which ? u : g;
-        const T *bias = static_cast<const T *>(which ? ep.bias2 : ep.bias);
-        T *Z = static_cast<T *>(which ? ep.Z2 : ep.Z) + m * (which ? ep.ldZ2 : ep.ldZ) + n;
+    if constexpr (FULL) {
+        const T *bias = static_cast<const T *>(ep.bias), *res = static_cast<const T *>(ep.R);
+        T *Z = static_cast<T *>(ep.Z);
+        float t[R];
         if (bias) {
-            float t[R];
-            if constexpr (R % 4 == 0)
-                if (whole) run_load(bias + n, t);
-            if (!whole) {
-#pragma unroll
-                for (int e = 0; e < R; e++) t[e] = n + e < N ? dense_load(bias + n + e) : 0.f;
-            }
+            run_load(bias + n, t);
 #pragma unroll
             for (int e = 0; e < R; e++) v[e] += t[e];
         }
-        if (which ? ep.Z2 != nullptr : ep.Z != nullptr) {
-            if constexpr (R % 4 == 0)
-                if (whole) run_store(Z, v);
-            if (!whole) {
+        if (Z) run_store(Z + m * ep.ldZ + n, v);
+        run_act<T>(ep.act, v, ep.slope);
+        if (res) {
+            run_load(res + m * ep.ldR + n, t);
 #pragma unroll
-                for (int e = 0; e < R; e++)
-                    if (n + e < N) dense_store(Z + e, v[e]);
-            }
+            for (int e = 0; e < R; e++) v[e] += t[e];
         }
     }
+    run_store(Y, v);
+}
+
+template <typename T, int R>
+static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &ep, float (&g)[R], float (&u)[R], long m, int n)
+{
+    const T *bg = static_cast<const T *>(ep.bias), *bu = static_cast<const T *>(ep.bias2);
+    T *G = static_cast<T *>(ep.Z), *U = static_cast<T *>(ep.Z2);
+    float t[R];
+    if (bg) {
+        run_load(bg + n, t);
+#pragma unroll
+        for (int e = 0; e < R; e++) g[e] += t[e];
+    }
+    if (bu) {
+        run_load(bu + n, t);
+#pragma unroll
+        for (int e = 0; e < R; e++) u[e] += t[e];
+    }
+    if (G) run_store(G + m * ep.ldZ + n, g);
+    if (U) run_store(U + m * ep.ldZ2 + n, u);
     run_act<T>(ep.act, g, ep.slope);
 #pragma unroll
     for (int e = 0; e < R; e++) g[e] *= u[e];
-    if constexpr (R % 4 == 0)
-        if (whole) run_store(Y, g);
-    if (!whole) {
-#pragma unroll
-        for (int e = 0; e < R; e++)
-            if (n + e < N) dense_store(Y + e, g[e]);
-    }
+    run_store(static_cast<T *>(ep.Y) + m * ep.ldY + n, g);
 }
 
 }  // namespace alpha

@@ -7,7 +7,7 @@ namespace alpha {
 
 // Adds the pieces of the cut tiles in their order and applies the epilogue: eight columns a thread, a workgroup 256 / (BN / 8)
 // rows of a tile (gated: BN / 16 threads a row, eight columns of each filter).
-template <typename T, bool GATED>
+template <typename T, bool GATED, bool FULL>
 __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a, int bm, int bn, long a_row, long a_k, long b_row, long b_k)
 {
     const int lanes = bn / (GATED ? 16 : 8), rows = 256 / lanes, per_tile = bm / rows;
@@ -45,8 +45,18 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
                 u[e] = dense_element(a.A[0], a.A[0], m * a_row, a_k, a.B[1], a.B[1], (n + e) * b_row, b_k, 1, a.K);
         }
     }
-    if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n, a.N);
-    else dense_finish<T>(a.ep, v, m, n, a.N);
+    if (a.ep.vec && n + 8 <= a.N) {
+        if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n);
+        else dense_finish<T, 8, FULL>(a.ep, v, m, n);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (n + e >= a.N) break;
+            float x[1] = {v[e]}, z[1] = {u[e]};
+            if constexpr (GATED) dense_finish_gated<T>(a.ep, x, z, m, n + e);
+            else dense_finish<T, 1, FULL>(a.ep, x, m, n + e);
+        }
+    }
 }
 
 namespace {
@@ -155,13 +165,10 @@ hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
     if (e != hipSuccess || cut == 0) return e;
     const dim3 grid((unsigned)cut * (unsigned)(bm * bn / (p.gated ? 16 : 8) / 256));
     const long a_row = p.a_t ? 1 : p.A.ld, a_k = p.a_t ? p.A.ld : 1, b_row = p.b_t ? 1 : p.B.ld, b_k = p.b_t ? p.B.ld : 1;
-    if (p.gated) {
-        if (p.f32) hipLaunchKernelGGL((dense_pieces_kernel<float, true>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
-        else hipLaunchKernelGGL((dense_pieces_kernel<__bf16, true>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
-    } else {
-        if (p.f32) hipLaunchKernelGGL((dense_pieces_kernel<float, false>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
-        else hipLaunchKernelGGL((dense_pieces_kernel<__bf16, false>), grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k);
-    }
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k); };
+    if (p.gated) p.f32 ? launch(dense_pieces_kernel<float, true, true>) : launch(dense_pieces_kernel<__bf16, true, true>);
+    else if (p.b_t) p.f32 ? launch(dense_pieces_kernel<float, false, false>) : launch(dense_pieces_kernel<__bf16, false, false>);
+    else p.f32 ? launch(dense_pieces_kernel<float, false, true>) : launch(dense_pieces_kernel<__bf16, false, true>);
     return hipGetLastError();
 }
 

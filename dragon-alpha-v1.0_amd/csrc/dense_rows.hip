@@ -85,10 +85,15 @@ hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_l
     return f32 ? launch_pack<float>(s, src, src_ld, total, cols, dst, ld) : launch_pack<__bf16>(s, src, src_ld, total, cols, dst, ld);
 }
 
-// A workgroup takes 256 columns (32 lanes of 8) of a run of rows, eight rows at a time; its column sums go to sums[run].
-template <typename T, bool VEC, bool GATED>
+constexpr int DELTA_ROWS = 4;
+
+// A workgroup takes 256 columns (32 lanes of 8) of a run of rows, eight rows side by side; its column sums go to sums[run], or, of
+// a single run, where they are wanted.
+// (A kernel per activation: with all of them behind a switch the code was 17 to 44 KB, and a small call the time of fetching it.)
+template <typename T, bool VEC, bool GATED, int ACT>
 __global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, long rows_per)
 {
+    constexpr int ROWS = sizeof(T) == 4 && ACT == ALPHA_DENSE_ACT_GELU ? 2 : DELTA_ROWS;   // (erf is long)
     __shared__ float part[GATED ? 2 : 1][8][257];
     const int lane = threadIdx.x & 31, ry = threadIdx.x >> 5, c = (blockIdx.x * 32 + lane) * 8;
     const long r0 = (long)blockIdx.y * rows_per, r1 = r0 + rows_per < d.rows ? r0 + rows_per : d.rows;
@@ -96,30 +101,41 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, lo
 #pragma unroll
     for (int e = 0; e < 8; e++) sum[e] = sum2[e] = 0.f;
     if (c < d.ld) {
-        for (long r = r0 + ry; r < r1; r += 8) {
-            float dy[8], z[8], u[8], out2[8];
-            load8<T, VEC>(static_cast<const T *>(d.dY) + r * d.ldY, c, d.cols, dy);
-            if (GATED || d.act != ALPHA_DENSE_ACT_NONE) load8<T, VEC>(static_cast<const T *>(d.Z) + r * d.ldZ, c, d.cols, z);
-            if constexpr (GATED) load8<T, VEC>(static_cast<const T *>(d.U) + r * d.ldU, c, d.cols, u);
+        // ROWS rows of a lane at a time: their loads first, then the arithmetic
+        for (long r = r0 + ry; r < r1; r += 8 * ROWS) {
+            float dy[ROWS][8], z[ROWS][8], u[ROWS][8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if (c + e >= d.cols) {   // pad columns: zeros, whatever act(0) is
-                    dy[e] = out2[e] = 0.f;
-                } else if constexpr (GATED) {
-                    out2[e] = dy[e] * dense_act<T>(d.act, z[e], d.slope);
-                    dy[e] *= u[e] * dense_act_slope<T>(d.act, z[e], d.slope);
-                } else if (d.act != ALPHA_DENSE_ACT_NONE) {
-                    dy[e] *= dense_act_slope<T>(d.act, z[e], d.slope);
-                }
-                sum[e] += dy[e];
-                if constexpr (GATED) sum2[e] += out2[e];
+            for (int y = 0; y < ROWS; y++) {
+                const long row = r + 8 * y < r1 ? r + 8 * y : r;
+                load8<T, VEC>(static_cast<const T *>(d.dY) + row * d.ldY, c, d.cols, dy[y]);
+                if (GATED || ACT != ALPHA_DENSE_ACT_NONE) load8<T, VEC>(static_cast<const T *>(d.Z) + row * d.ldZ, c, d.cols, z[y]);
+                if constexpr (GATED) load8<T, VEC>(static_cast<const T *>(d.U) + row * d.ldU, c, d.cols, u[y]);
             }
-            if (d.dst) store8(static_cast<T *>(d.dst) + r * d.ld2 + c, dy);
-            if constexpr (GATED)
-                if (d.dst2) store8(static_cast<T *>(d.dst2) + r * d.ld2 + c, out2);
+#pragma unroll
+            for (int y = 0; y < ROWS; y++) {
+                const long row = r + 8 * y;
+                if (row >= r1) break;
+                float out2[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (c + e >= d.cols) {   // pad columns: zeros, whatever act(0) is
+                        dy[y][e] = out2[e] = 0.f;
+                    } else if constexpr (GATED) {
+                        out2[e] = dy[y][e] * dense_act<T>(ACT, z[y][e], d.slope);
+                        dy[y][e] *= u[y][e] * dense_act_slope<T>(ACT, z[y][e], d.slope);
+                    } else if (ACT != ALPHA_DENSE_ACT_NONE) {
+                        dy[y][e] *= dense_act_slope<T>(ACT, z[y][e], d.slope);
+                    }
+                    sum[e] += dy[y][e];
+                    if constexpr (GATED) sum2[e] += out2[e];
+                }
+                if (d.dst) store8(static_cast<T *>(d.dst) + row * d.ld2 + c, dy[y]);
+                if constexpr (GATED)
+                    if (d.dst2) store8(static_cast<T *>(d.dst2) + row * d.ld2 + c, out2);
+            }
         }
     }
-    if (!d.sums) return;
+    if (!d.dB && !d.dB2) return;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         part[0][ry][lane * 8 + e] = sum[e];
@@ -133,7 +149,11 @@ __global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, lo
         float t = 0.f;
 #pragma unroll
         for (int y = 0; y < 8; y++) t += part[w][y][threadIdx.x];
-        d.sums[((long)blockIdx.y * (GATED ? 2 : 1) + w) * d.cols + col] = t;
+        if (gridDim.y > 1) {
+            d.sums[((long)blockIdx.y * (GATED ? 2 : 1) + w) * d.cols + col] = t;
+        } else if (void *dB = w ? d.dB2 : d.dB) {   // one run: the sums are final
+            dense_store(static_cast<T *>(dB) + col, t);
+        }
     }
 }
 
@@ -159,12 +179,27 @@ __global__ __launch_bounds__(256) void dense_delta_sum_kernel(const float *__res
 
 namespace {
 
-// Runs of rows: enough workgroups for the device, at least 32 rows each (a run costs a row of sums), at most 256 runs.
+// Runs of rows: enough workgroups for the device, whole turns of 8 * DELTA_ROWS rows, at most 256 (a run costs a row of sums); up
+// to two turns one run, whose sums need no second kernel.
 long delta_rows_per(long rows, int cols)
 {
+    const long turn = 8 * DELTA_ROWS;
+    if (rows <= 2 * turn) return std::max<long>(1, rows);
     const long blocks_x = (cols + 255) / 256, want = std::max<long>(1, 2048 / std::max<long>(1, blocks_x));
-    const long runs = std::min<long>(256, std::max<long>(1, std::min(want, rows / 32)));
-    return std::max<long>(1, (rows + runs - 1) / runs);
+    const long runs = std::min<long>(256, std::max<long>(1, std::min(want, rows / turn))), per = (rows + runs - 1) / runs;
+    return (per + turn - 1) / turn * turn;
+}
+
+template <typename T, bool VEC, bool GATED>
+void launch_delta_act(hipStream_t s, const DenseDelta &d, dim3 grid, long rows_per)
+{
+    switch (d.act) {
+    case ALPHA_DENSE_ACT_LEAKY_RELU: hipLaunchKernelGGL((dense_delta_kernel<T, VEC, GATED, ALPHA_DENSE_ACT_LEAKY_RELU>), grid, dim3(256), 0, s, d, rows_per); break;
+    case ALPHA_DENSE_ACT_GELU: hipLaunchKernelGGL((dense_delta_kernel<T, VEC, GATED, ALPHA_DENSE_ACT_GELU>), grid, dim3(256), 0, s, d, rows_per); break;
+    case ALPHA_DENSE_ACT_SILU: hipLaunchKernelGGL((dense_delta_kernel<T, VEC, GATED, ALPHA_DENSE_ACT_SILU>), grid, dim3(256), 0, s, d, rows_per); break;
+    case ALPHA_DENSE_ACT_SIGMOID: hipLaunchKernelGGL((dense_delta_kernel<T, VEC, GATED, ALPHA_DENSE_ACT_SIGMOID>), grid, dim3(256), 0, s, d, rows_per); break;
+    default: hipLaunchKernelGGL((dense_delta_kernel<T, VEC, GATED, ALPHA_DENSE_ACT_NONE>), grid, dim3(256), 0, s, d, rows_per); break;
+    }
 }
 
 template <typename T>
@@ -173,13 +208,14 @@ hipError_t launch_delta_typed(hipStream_t s, const DenseDelta &d, bool vec, long
     const dim3 grid((unsigned)((d.ld + 255) / 256), (unsigned)std::max(runs, 1));
     if (runs > 0) {
         if (d.gated) {
-            if (vec) hipLaunchKernelGGL((dense_delta_kernel<T, true, true>), grid, dim3(256), 0, s, d, rows_per);
-            else hipLaunchKernelGGL((dense_delta_kernel<T, false, true>), grid, dim3(256), 0, s, d, rows_per);
+            if (vec) launch_delta_act<T, true, true>(s, d, grid, rows_per);
+            else launch_delta_act<T, false, true>(s, d, grid, rows_per);
         } else {
-            if (vec) hipLaunchKernelGGL((dense_delta_kernel<T, true, false>), grid, dim3(256), 0, s, d, rows_per);
-            else hipLaunchKernelGGL((dense_delta_kernel<T, false, false>), grid, dim3(256), 0, s, d, rows_per);
+            if (vec) launch_delta_act<T, true, false>(s, d, grid, rows_per);
+            else launch_delta_act<T, false, false>(s, d, grid, rows_per);
         }
     }
+    if (runs == 1) return hipGetLastError();
     const dim3 cols((unsigned)((d.cols + 15) / 16));
     const int of = d.gated ? 2 : 1;
     if (d.dB) hipLaunchKernelGGL((dense_delta_sum_kernel<T>), cols, dim3(256), 0, s, d.sums, runs, d.cols, 0, of, static_cast<T *>(d.dB));
@@ -193,14 +229,13 @@ size_t dense_delta_sum_bytes(long rows, int cols, int gated)
 {
     if (rows <= 0 || cols <= 0) return 0;
     const long per = delta_rows_per(rows, cols), runs = (rows + per - 1) / per;
-    return (size_t)runs * cols * (gated ? 2 : 1) * 4;
+    return runs > 1 ? (size_t)runs * cols * (gated ? 2 : 1) * 4 : 0;
 }
 
 hipError_t launch_dense_delta(hipStream_t s, const DenseDelta &given)
 {
     DenseDelta d = given;
     if (d.cols <= 0) return hipSuccess;
-    if (!d.dB && !d.dB2) d.sums = nullptr;
     const long per = delta_rows_per(d.rows, d.cols), runs = d.rows > 0 ? (d.rows + per - 1) / per : 0;
     auto fits = [&](const void *p, long ld) { return (reinterpret_cast<uintptr_t>(p) & (d.f32 ? 15 : 7)) == 0 && (ld & 3) == 0; };
     const bool vec = fits(d.dY, d.ldY) && fits(d.Z, d.ldZ) && fits(d.U, d.ldU);

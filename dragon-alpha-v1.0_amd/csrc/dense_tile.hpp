@@ -91,6 +91,7 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
                                                 int wn, int m0, int n0, bool cut, int piece, int cut_tile, int cut_tiles)
 {
     constexpr int TM = BM / WM, TN = BN / WN, MF = TM / 16;
+    constexpr bool FULL = !BT;     // B with k as its rows: a backward's product
     const int l16 = lane & 15, q = lane >> 4;
     constexpr int ROW = 68;                              // floats from row to row: 16 bytes past a multiple of the banks
     constexpr int LANES = GATED ? 4 : 8;                 // lanes of a row, eight columns each (gated: eight of each filter)
@@ -99,62 +100,80 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
     static_assert(WM * WN * 32 * ROW * 4 <= LDS, "the tiles' buffers hold the parts");
     float *const part = reinterpret_cast<float *>(smem) + wave * (32 * ROW);
     const int at = (lane % LANES) * 8, n = n0 + wn * (GATED ? 32 : 64) + at;
+    // The turns over pairs of fragment rows are not unrolled (only their copies out of the registers are): a workgroup runs
+    // this once, and what it costs is largely the fetching of its code.
+    const bool vec = a.ep.vec;
     unsigned again = 0;   // fp32: runs with a NaN among them, computed once more below
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < MF; i += 2) {
+        for_each<MF / 2>([&](auto pair) __attribute__((always_inline)) {
+            if (i == 2 * pair) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[i + h][j];
+                    for (int j = 0; j < 4; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[2 * pair + h][j];
+            }
+        });
         wave_fence();
 #pragma unroll 1
         for (int y = 0; y < 32; y += AT_ONCE) {
             const int row = y + lane / LANES;
             const long m = m0 + wm * TM + i * 16 + row;
+            const float *src = part + row * ROW + at;
             float v[8], u[8];
-            run_load(part + row * ROW + at, v);
-            if constexpr (GATED) run_load(part + row * ROW + 32 + at, u);
+            run_load(src, v);
+            if constexpr (GATED) run_load(src + 32, u);
             if (m >= a.M || n >= a.N) continue;
             if (cut) {
                 float *dst = a.pieces + (((long)piece * cut_tiles + cut_tile) * BM + (wm * TM + i * 16 + row)) * BN + wn * TN + at;
                 run_store(dst, v);
                 if constexpr (GATED) run_store(dst + 32, u);
-            } else {
-                if constexpr (__is_same(T, float)) {
-                    float sum = 0.f;
+                continue;
+            }
+            if constexpr (__is_same(T, float)) {
+                float sum = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
-                    if (sum != sum) {   // (also where infinities of both signs meet: no harm)
-                        again |= 1u << (i / 2 * TURNS + y / AT_ONCE);
-                        continue;
-                    }
+                for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
+                if (sum != sum) {   // (also where infinities of both signs meet: no harm)
+                    again |= 1u << (i / 2 * TURNS + y / AT_ONCE);
+                    continue;
                 }
-                if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n, a.N);
-                else dense_finish<T>(a.ep, v, m, n, a.N);
+            }
+            if (vec && n + 8 <= a.N) {
+                if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n);
+                else dense_finish<T, 8, FULL>(a.ep, v, m, n);
+            } else {
+#pragma unroll 1
+                for (int e = 0; e < 8 && n + e < a.N; e++) {
+                    float x[1] = {src[e]}, z[1] = {GATED ? src[32 + e] : 0.f};
+                    if constexpr (GATED) dense_finish_gated<T>(a.ep, x, z, m, n + e);
+                    else dense_finish<T, 1, FULL>(a.ep, x, m, n + e);
+                }
             }
         }
         wave_fence();
     }
     if constexpr (__is_same(T, float)) {
         static_assert(MF / 2 * TURNS <= 32, "one bit per run");
+#pragma unroll 1
         while (again) {
             const int bit = __ffs(again) - 1;
             again &= again - 1;
             const long m = m0 + wm * TM + bit / TURNS * 32 + bit % TURNS * AT_ONCE + lane / LANES;
+#pragma unroll 1
             for (int e = 0; e < 8 && n + e < a.N; e++) {
-                float v[1], u[1] = {0.f};
-                v[0] = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.B[0], a.B[1], BT ? n + e : (n + e) * a.ldB,
+                float x[1], z[1] = {0.f};
+                x[0] = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.B[0], a.B[1], BT ? n + e : (n + e) * a.ldB,
                                      BT ? a.ldB : 1, GATED ? 1 : a.sources, a.K);
                 if constexpr (GATED) {
-                    u[0] = dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.B[1], a.B[1], (n + e) * a.ldB, 1, 1, a.K);
-                    dense_finish_gated<T>(a.ep, v, u, m, n + e, a.N);
+                    z[0] = dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.B[1], a.B[1], (n + e) * a.ldB, 1, 1, a.K);
+                    dense_finish_gated<T>(a.ep, x, z, m, n + e);
                 } else {
-                    dense_finish<T>(a.ep, v, m, n + e, a.N);
+                    dense_finish<T, 1, FULL>(a.ep, x, m, n + e);
                 }
             }
         }
     }
 }
-
 
 }  // namespace alpha
