@@ -30,23 +30,18 @@ __device__ __forceinline__ typename FewVec<T>::type few_load(const T *row, int k
     __builtin_memcpy(&v, row + k, 16);
     return v;
 }
-// the same with zeros from K on
+// what was loaded at K - V instead of at k > K - V, moved to its place: zeros from K on
 template <typename T>
-__device__ __forceinline__ typename FewVec<T>::type few_load_tail(const T *row, int k, int K)
+__device__ __forceinline__ typename FewVec<T>::type few_at_edge(typename FewVec<T>::type x, int k, int K)
 {
     constexpr int V = 16 / sizeof(T);
     T v[V];
-    if (K >= V) {   // uniform
-        load_columns<V>(row, k, K, v);
-        at_edge<V>(k, K, v);
-    } else {
 #pragma unroll
-        for (int e = 0; e < V; e++) v[e] = k + e < K ? row[k + e] : (T)0.f;
-    }
-    typename FewVec<T>::type out;
+    for (int e = 0; e < V; e++) v[e] = x[e];
+    at_edge<V>(k, K, v);
 #pragma unroll
-    for (int e = 0; e < V; e++) out[e] = v[e];
-    return out;
+    for (int e = 0; e < V; e++) x[e] = v[e];
+    return x;
 }
 
 __device__ __forceinline__ floatx4 few_multiply(bf16x8 w, bf16x8 x, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
@@ -87,40 +82,58 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
 
     // Every workgroup starts at another place of the reduction: rows are often a power of two apart, and workgroups that
     // all read the same k at a time would all ask the same few channels of the memory.
-    const int turns = (a.K + FEW_WAVES * SPAN - 1) / (FEW_WAVES * SPAN);
+    const int turns = a.K < V ? 0 : (a.K + FEW_WAVES * SPAN - 1) / (FEW_WAVES * SPAN);
     int turn = turns > 0 ? (int)(blockIdx.x % turns) : 0;
     for (int t = 0; t < turns; t++) {
         const int k0 = (turn * FEW_WAVES + wave) * SPAN, k = k0 + l16 / C * PIECE;
-        vec vw[G][4], vx[MB][4];
-        if (k0 + SPAN <= a.K) {
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-                for (int g = 0; g < G; g++) vw[g][c] = few_load(w[g], k + c * CHUNK + q * V);
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-                for (int b = 0; b < MB; b++) vx[b][c] = few_load(x[b], k + c * CHUNK + q * V);
-        } else if (k0 < a.K) {
+        if (k0 < a.K) {
+            vec vw[G][4], vx[MB][4];
+            const int last = a.K - V;      // >= 0
 #pragma unroll
             for (int c = 0; c < 4; c++) {
+                const int at = k + c * CHUNK + q * V;
 #pragma unroll
-                for (int g = 0; g < G; g++) vw[g][c] = few_load_tail(w[g], k + c * CHUNK + q * V, a.K);
-#pragma unroll
-                for (int b = 0; b < MB; b++) vx[b][c] = few_load_tail(x[b], k + c * CHUNK + q * V, a.K);
+                for (int g = 0; g < G; g++) vw[g][c] = few_load(w[g], at < last ? at : last);
             }
-        }
-        if (k0 < a.K) {
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 4; c++) {
+                const int at = k + c * CHUNK + q * V;
+#pragma unroll
+                for (int b = 0; b < MB; b++) vx[b][c] = few_load(x[b], at < last ? at : last);
+            }
+            const bool edge = k0 + SPAN > a.K;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (edge) {
+#pragma unroll
+                    for (int g = 0; g < G; g++) vw[g][c] = few_at_edge<T>(vw[g][c], k + c * CHUNK + q * V, a.K);
+#pragma unroll
+                    for (int b = 0; b < MB; b++) vx[b][c] = few_at_edge<T>(vx[b][c], k + c * CHUNK + q * V, a.K);
+                }
 #pragma unroll
                 for (int g = 0; g < G; g++)
 #pragma unroll
                     for (int b = 0; b < MB; b++) acc[g][b] = few_multiply(vw[g][c], vx[b][c], acc[g][b]);
+            }
         }
         turn = turn + 1 == turns ? 0 : turn + 1;
     }
 
+    if (a.K < V && wave == 0) {   // less than one load: element by element, zeros behind and in the other lanes' pieces
+        vec vw[G], vx[MB];
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const bool there = e < a.K && q == 0 && l16 < C;
+#pragma unroll
+            for (int g = 0; g < G; g++) vw[g][e] = there ? w[g][e] : (T)0.f;
+#pragma unroll
+            for (int b = 0; b < MB; b++) vx[b][e] = there ? x[b][e] : (T)0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int b = 0; b < MB; b++) acc[g][b] = few_multiply(vw[g], vx[b], acc[g][b]);
+    }
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
@@ -140,8 +153,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
                 v[0] += reinterpret_cast<const float *>(&part[s][b][at])[col & 3];
                 if constexpr (GATED) u[0] += reinterpret_cast<const float *>(&part[s][(GATED ? MB : 0) + b][at])[col & 3];
             }
-        if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n0 + col);
-        else dense_finish<T, 1, true>(a.ep, v, m, n0 + col);
+        if constexpr (GATED) dense_finish_gated<T, 1, false>(a.ep, v, u, m, n0 + col);
+        else dense_finish<T, 1, true, false>(a.ep, v, m, n0 + col);
     }
 }
 

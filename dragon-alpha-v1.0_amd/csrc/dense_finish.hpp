@@ -4,12 +4,10 @@
 
 namespace alpha {
 
-// R consecutive elements of a row, aligned to groups of four, or one element.
+// R consecutive elements of a row, aligned to groups of four.
 template <int R, typename T>
 static __device__ __forceinline__ void run_load(const T *p, float (&v)[R])
 {
-    if constexpr (R == 1) v[0] = dense_load(p);
-    else
 #pragma unroll
     for (int i = 0; i < R; i += 4) {
         const floatx4 q = quad_load(p + i);
@@ -20,9 +18,7 @@ static __device__ __forceinline__ void run_load(const T *p, float (&v)[R])
 template <int R, typename T>
 static __device__ __forceinline__ void run_store(T *p, const float (&v)[R])
 {
-    if constexpr (R == 1) {
-        dense_store(p, v[0]);
-    } else if constexpr (R == 8 && sizeof(T) == 2) {   // one 128-bit store (the hardware takes 8-byte alignment)
+    if constexpr (R == 8 && sizeof(T) == 2) {   // one 128-bit store (the hardware takes 8-byte alignment)
         bf16x8 q;
 #pragma unroll
         for (int e = 0; e < 8; e++) q[e] = (T)v[e];
@@ -56,56 +52,86 @@ static __device__ __forceinline__ void run_act(int act, float (&v)[R], float k)
     }
 }
 
-// The epilogues of R consecutive columns n .. n+R-1 of row m, R a multiple of four and aligned to it, or one element. FULL: all
-// of the epilogue; else only the store (the products of a backward).
-template <typename T, int R, bool FULL>
-static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n)
+// The same for the `left` first of R elements at any address.
+template <int R, typename T>
+static __device__ __forceinline__ void edge_load(const T *p, int left, float (&v)[R])
+{
+#pragma unroll
+    for (int e = 0; e < R; e++) v[e] = dense_load(p + (e < left ? e : left - 1));
+}
+template <int R, typename T>
+static __device__ __forceinline__ void edge_store(T *p, int left, const float (&v)[R])
+{
+#pragma unroll
+    for (int e = 0; e < R; e++)
+        if (e < left) dense_store(p + e, v[e]);
+}
+
+// The epilogues of R consecutive columns n .. n+R-1 of row m. WHOLE: all of them exist and groups of four are aligned; else the
+// `left` first. FULL: all of the epilogue; else only the store (the products of a backward).
+template <typename T, int R, bool FULL, bool WHOLE>
+static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n, int left = R)
 {
     const bool second = !FULL && ep.row2 > 0 && m >= ep.row2;
     if (!FULL && ep.row2 > 0 && !second && m >= ep.rows1) return;   // a row between two stacked products
     T *Y = static_cast<T *>(second ? ep.Y2 : ep.Y) + (second ? (m - ep.row2) * ep.ldY2 : m * ep.ldY) + n;
+    auto load = [&](const T *p, float (&t)[R]) {
+        if constexpr (WHOLE) run_load(p, t);
+        else edge_load(p, left, t);
+    };
+    auto store = [&](T *p, const float (&t)[R]) {
+        if constexpr (WHOLE) run_store(p, t);
+        else edge_store(p, left, t);
+    };
     if constexpr (FULL) {
         const T *bias = static_cast<const T *>(ep.bias), *res = static_cast<const T *>(ep.R);
         T *Z = static_cast<T *>(ep.Z);
-        float t[R];
+        float t[R], r[R];
+        if (res) load(res + m * ep.ldR + n, r);
         if (bias) {
-            run_load(bias + n, t);
+            load(bias + n, t);
 #pragma unroll
             for (int e = 0; e < R; e++) v[e] += t[e];
         }
-        if (Z) run_store(Z + m * ep.ldZ + n, v);
+        if (Z) store(Z + m * ep.ldZ + n, v);
         run_act<T>(ep.act, v, ep.slope);
         if (res) {
-            run_load(res + m * ep.ldR + n, t);
 #pragma unroll
-            for (int e = 0; e < R; e++) v[e] += t[e];
+            for (int e = 0; e < R; e++) v[e] += r[e];
         }
     }
-    run_store(Y, v);
+    store(Y, v);
 }
 
-template <typename T, int R>
-static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &ep, float (&g)[R], float (&u)[R], long m, int n)
+template <typename T, int R, bool WHOLE>
+static __device__ __forceinline__ void dense_finish_gated(const DenseEpilogue &ep, float (&g)[R], float (&u)[R], long m, int n, int left = R)
 {
-    const T *bg = static_cast<const T *>(ep.bias), *bu = static_cast<const T *>(ep.bias2);
-    T *G = static_cast<T *>(ep.Z), *U = static_cast<T *>(ep.Z2);
+    auto load = [&](const T *p, float (&t)[R]) {
+        if constexpr (WHOLE) run_load(p, t);
+        else edge_load(p, left, t);
+    };
+    auto store = [&](void *p, long ld, const float (&t)[R]) {
+        T *const q = static_cast<T *>(p) + m * ld + n;
+        if constexpr (WHOLE) run_store(q, t);
+        else edge_store(q, left, t);
+    };
     float t[R];
-    if (bg) {
-        run_load(bg + n, t);
+    if (ep.bias) {
+        load(static_cast<const T *>(ep.bias) + n, t);
 #pragma unroll
         for (int e = 0; e < R; e++) g[e] += t[e];
     }
-    if (bu) {
-        run_load(bu + n, t);
+    if (ep.bias2) {
+        load(static_cast<const T *>(ep.bias2) + n, t);
 #pragma unroll
         for (int e = 0; e < R; e++) u[e] += t[e];
     }
-    if (G) run_store(G + m * ep.ldZ + n, g);
-    if (U) run_store(U + m * ep.ldZ2 + n, u);
+    if (ep.Z) store(ep.Z, ep.ldZ, g);
+    if (ep.Z2) store(ep.Z2, ep.ldZ2, u);
     run_act<T>(ep.act, g, ep.slope);
 #pragma unroll
     for (int e = 0; e < R; e++) g[e] *= u[e];
-    run_store(static_cast<T *>(ep.Y) + m * ep.ldY + n, g);
+    store(ep.Y, ep.ldY, g);
 }
 
 }  // namespace alpha

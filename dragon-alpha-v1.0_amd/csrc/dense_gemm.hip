@@ -46,16 +46,12 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
         }
     }
     if (a.ep.vec && n + 8 <= a.N) {
-        if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n);
-        else dense_finish<T, 8, FULL>(a.ep, v, m, n);
+        if constexpr (GATED) dense_finish_gated<T, 8, true>(a.ep, v, u, m, n);
+        else dense_finish<T, 8, FULL, true>(a.ep, v, m, n);
     } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if (n + e >= a.N) break;
-            float x[1] = {v[e]}, z[1] = {u[e]};
-            if constexpr (GATED) dense_finish_gated<T>(a.ep, x, z, m, n + e);
-            else dense_finish<T, 1, FULL>(a.ep, x, m, n + e);
-        }
+        const int left = a.N - n < 8 ? a.N - n : 8;
+        if constexpr (GATED) dense_finish_gated<T, 8, false>(a.ep, v, u, m, n, left);
+        else dense_finish<T, 8, FULL, false>(a.ep, v, m, n, left);
     }
 }
 

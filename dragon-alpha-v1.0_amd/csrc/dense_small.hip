@@ -131,14 +131,9 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
         for (int w = 0; w < SMALL_WAVES; w++) v[j] += reinterpret_cast<const float *>(&part[w][t * 4 + j][at])[i & 3];
     }
     if (a.ep.vec && n + 4 <= a.N) {
-        dense_finish<T, 4, false>(a.ep, v, m, n);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (n + j >= a.N) break;
-        float one[1] = {v[j]};
-        dense_finish<T, 1, false>(a.ep, one, m, n + j);
+        dense_finish<T, 4, false, true>(a.ep, v, m, n);
+    } else {
+        dense_finish<T, 4, false, false>(a.ep, v, m, n, a.N - n < 4 ? a.N - n : 4);
     }
 }
 

@@ -140,15 +140,12 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
                 }
             }
             if (vec && n + 8 <= a.N) {
-                if constexpr (GATED) dense_finish_gated<T>(a.ep, v, u, m, n);
-                else dense_finish<T, 8, FULL>(a.ep, v, m, n);
+                if constexpr (GATED) dense_finish_gated<T, 8, true>(a.ep, v, u, m, n);
+                else dense_finish<T, 8, FULL, true>(a.ep, v, m, n);
             } else {
-#pragma unroll 1
-                for (int e = 0; e < 8 && n + e < a.N; e++) {
-                    float x[1] = {src[e]}, z[1] = {GATED ? src[32 + e] : 0.f};
-                    if constexpr (GATED) dense_finish_gated<T>(a.ep, x, z, m, n + e);
-                    else dense_finish<T, 1, FULL>(a.ep, x, m, n + e);
-                }
+                const int left = a.N - n < 8 ? a.N - n : 8;
+                if constexpr (GATED) dense_finish_gated<T, 8, false>(a.ep, v, u, m, n, left);
+                else dense_finish<T, 8, FULL, false>(a.ep, v, m, n, left);
             }
         }
         wave_fence();
@@ -167,9 +164,9 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
                                      BT ? a.ldB : 1, GATED ? 1 : a.sources, a.K);
                 if constexpr (GATED) {
                     z[0] = dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.B[1], a.B[1], (n + e) * a.ldB, 1, 1, a.K);
-                    dense_finish_gated<T>(a.ep, x, z, m, n + e);
+                    dense_finish_gated<T, 1, false>(a.ep, x, z, m, n + e);
                 } else {
-                    dense_finish<T, 1, FULL>(a.ep, x, m, n + e);
+                    dense_finish<T, 1, FULL, false>(a.ep, x, m, n + e);
                 }
             }
         }
