@@ -8,7 +8,7 @@
 // the last are the last once more, their results not stored. The partial sums are added through LDS in a fixed order.
 // At most four rows of X: four columns a workgroup instead of 16, the MFMA's 16 rows and columns being four pieces of the
 // reduction times four (only the products of equal pieces are read out): four times as many workgroups, each with a
-// quarter of the reduction's length in turns (1 x 8192 x 1024: 11.4 -> 6.5 us).
+// quarter of the reduction's length in turns (1 x 8192 x 1024 of bf16: 11.4 -> 5.4 us).
 // Rows may begin at any element and K may be any number.
 #include "dense_finish.hpp"
 
@@ -160,11 +160,22 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
 
 namespace {
 
+// Four columns a workgroup or 16, for at most four rows: 16 where the columns make a workgroup per compute unit anyway and four
+// would leave wavefronts without a piece of the reduction, if it is one turn, or a pair of filters to read (bf16, us, 4 / 16
+// columns: 1024 -> 4096 3.8 / 3.3, pair 2048 -> 8192 16.0 / 12.6; 2048 -> 8192 7.8 / 8.5, 4096 -> 4096 7.6 / 8.6, 8192 -> 512 4.7 / 10.6).
+template <typename T>
+bool few_columns(const DenseFewRows &a)
+{
+    constexpr int TURN = FEW_WAVES * 4 * 64 / sizeof(T);     // of 16 columns; of four, four times as long
+    const bool filled = (a.N + 15) / 16 >= device_cu_count(), idle = a.K < 4 * TURN;
+    return !(filled && idle && (a.gated || a.K <= TURN));
+}
+
 template <typename T, bool GATED>
 hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
 {
     const dim3 block(FEW_WAVES * 64), grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 63) / 64));
-    if (a.M <= 4) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 1, 4>), dim3((unsigned)((a.N + 3) / 4)), block, 0, s, a);
+    if (a.M <= 4 && few_columns<T>(a)) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 1, 4>), dim3((unsigned)((a.N + 3) / 4)), block, 0, s, a);
     else if (a.M <= 16) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 1, 16>), grid, block, 0, s, a);
     else if (a.M <= 32) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 2, 16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 4, 16>), grid, block, 0, s, a);
