@@ -191,6 +191,7 @@ hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
 bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K)
 {
     if (M <= 16) return true;
+    if ((M + 63) / 64 > 65535) return false;   // (the grid's second dimension)
     static constexpr double bf16_turn[2] = {2.7, 4.7}, f32_turn[2] = {2.7, 5.3};
     const int cus = device_cu_count() > 0 ? device_cu_count() : 1;
     const long groups = (long)((N + 15) / 16) * ((M + 63) / 64), rounds = (groups + cus - 1) / cus;
