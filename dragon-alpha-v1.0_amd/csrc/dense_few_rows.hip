@@ -185,18 +185,18 @@ hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
 }  // namespace
 
 // Up to 16 rows always: W is the time, and this kernel reads it once and as it is. More rows: by an estimate against the tile
-// kernel's. A workgroup's turn (1024 k of bf16, 512 of fp32) of 1 / 2 / 4 blocks of rows takes 1.3 / 2.7 / 4.7 us in bf16,
-// 1.8 / 2.7 / 5.3 in fp32 (measured on 4096 x 4096 and 8192 x 1024 filters), 1.4 times that for a gated pair. E.g. 200 rows
-// of 512 x 1000 bf16: 5.4 us here, 9 to 18 through tiles; 128 rows of 4096 x 4096: 39 against 20.
+// kernel's. A workgroup's turn (1024 k of bf16, 512 of fp32) of 2 / 4 blocks of rows takes 2.7 / 4.7 us in bf16, 2.7 / 6.5 in
+// fp32, 1.4 and 1.6 times that for a gated pair (measured on 512 x 1000 to 4096 x 4096 filters). E.g. 200 rows of 512 x 1000
+// bf16: 5.4 us here, 9 to 18 through tiles; 128 rows of 4096 x 4096: 39 against 20.
 bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K)
 {
     if (M <= 16) return true;
     if ((M + 63) / 64 > 65535) return false;   // (the grid's second dimension)
-    static constexpr double bf16_turn[2] = {2.7, 4.7}, f32_turn[2] = {2.7, 5.3};
+    static constexpr double turn_us[2][2] = {{2.7, 4.7}, {2.7, 6.5}};
     const int cus = device_cu_count() > 0 ? device_cu_count() : 1;
-    const long groups = (long)((N + 15) / 16) * ((M + 63) / 64), rounds = (groups + cus - 1) / cus;
-    const double turns = (double)K / (f32 ? 512 : 1024), turn = (f32 ? f32_turn : bf16_turn)[M > 32];
-    const double us = 2.0 + rounds * (turns < 0.6 ? 0.6 : turns) * turn * (gated ? 1.4 : 1.0);
+    const double groups = (double)((N + 15) / 16) * ((M + 63) / 64), turns = (double)K / (f32 ? 512 : 1024);
+    const double turn = turn_us[f32 ? 1 : 0][M > 32] * (!gated ? 1.0 : f32 ? 1.6 : 1.4);
+    const double us = 2.0 + (groups > cus ? groups / cus : 1.0) * (0.7 + (turns < 0.5 ? 0.5 : turns) * turn);
     return us < dense_product_us(M, N, K, f32, 1, gated);
 }
 

@@ -137,13 +137,13 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
     }
 }
 
-// By an estimate against the tile kernels': a workgroup's reduction takes 8.5 ns a k in fp32 (its MFMAs), 0.9 us a turn of 256 k
-// in bf16 (the loads). 100 x 2000 x 500 backward in fp32 / bf16: 14 + 14 / 13 + 8 us through tiles, 7 + 5 / 5 + 4 here.
+// By an estimate against the tile kernels': a workgroup's reduction takes 12.5 ns a k in fp32 (its MFMAs), 0.9 us a turn of 256 k
+// in bf16 (the loads). 100 x 2000 x 500 backward in fp32 / bf16: 14 + 14 / 13 + 8 us through tiles, 10 + 8 / 7 + 5 here.
 bool dense_small_preferred(int f32, int M, int N, int K, int sources)
 {
     const int cus = device_cu_count() > 0 ? device_cu_count() : 1;
     const long groups = ((long)M + SMALL_M - 1) / SMALL_M * ((N + SMALL_N - 1) / SMALL_N), rounds = (groups + cus - 1) / cus;
-    const double all = (double)K * sources, us = 3.0 + rounds * (1.5 + (f32 ? all * 0.0085 : (double)(long)((all + 255) / 256) * 0.9));
+    const double all = (double)K * sources, us = 3.0 + rounds * (1.0 + (f32 ? all * 0.0125 : (double)(long)((all + 255) / 256) * 0.9));
     // (the loads at an edge take what lies before it)
     return M >= 2 && N >= 4 && K >= 8 && (M + SMALL_M - 1) / SMALL_M <= 65535 && us < dense_product_us(M, N, K, f32, sources, 0);
 }
