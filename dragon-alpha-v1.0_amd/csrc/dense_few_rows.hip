@@ -22,12 +22,26 @@ template <typename T> struct FewVec;
 template <> struct FewVec<float> { typedef floatx4 type; };
 template <> struct FewVec<__bf16> { typedef bf16x8 type; };
 
-// 16 bytes of a row from element k on, whatever its alignment
-template <typename T>
+// 16 bytes of a row from element k on, whatever its alignment. ODD: bf16 that may begin in the middle of a word, which the memory
+// pipe serves at a third of its rate (100 x 2001 x 500 28.0 -> 17.2 us); the words they lie in are loaded instead and shifted. (The
+// half word beside them is dropped: it shares its word, and so its page, with an element that is asked for.)
+template <bool ODD, typename T>
 __device__ __forceinline__ typename FewVec<T>::type few_load(const T *row, int k)
 {
     typename FewVec<T>::type v;
-    __builtin_memcpy(&v, row + k, 16);
+    if constexpr (ODD) {
+        const char *c = reinterpret_cast<const char *>(row + k);
+        const unsigned odd = (unsigned)reinterpret_cast<uintptr_t>(c) & 2;
+        c -= odd;
+        uint32_t w[5];
+        __builtin_memcpy(w, __builtin_assume_aligned(c, 4), 16);
+        __builtin_memcpy(w + 4, __builtin_assume_aligned(c + 12 + 2 * odd, 4), 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], odd * 8);
+        __builtin_memcpy(&v, w, 16);
+    } else {
+        __builtin_memcpy(&v, row + k, 16);
+    }
     return v;
 }
 // what was loaded at K - V instead of at k > K - V, moved to its place: zeros from K on
@@ -55,7 +69,7 @@ __device__ __forceinline__ floatx4 few_multiply(floatx4 w, floatx4 x, floatx4 c)
 }  // namespace
 
 // C: columns of a workgroup, 16, or 4 for at most four rows. MB: blocks of 16 rows.
-template <typename T, bool GATED, int MB, int C>
+template <typename T, bool ODD, bool GATED, int MB, int C>
 __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const DenseFewRows a)
 {
     typedef typename FewVec<T>::type vec;
@@ -93,13 +107,13 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
             for (int c = 0; c < 4; c++) {
                 const int at = k + c * CHUNK + q * V;
 #pragma unroll
-                for (int g = 0; g < G; g++) vw[g][c] = few_load(w[g], at < last ? at : last);
+                for (int g = 0; g < G; g++) vw[g][c] = few_load<ODD>(w[g], at < last ? at : last);
             }
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int at = k + c * CHUNK + q * V;
 #pragma unroll
-                for (int b = 0; b < MB; b++) vx[b][c] = few_load(x[b], at < last ? at : last);
+                for (int b = 0; b < MB; b++) vx[b][c] = few_load<ODD>(x[b], at < last ? at : last);
             }
             const bool edge = k0 + SPAN > a.K;
 #pragma unroll
@@ -160,6 +174,16 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
 
 namespace {
 
+// May a load of bf16 from these rows begin in the middle of a word?
+bool odd_rows(std::initializer_list<const void *> p, std::initializer_list<long> strides)
+{
+    for (const void *q : p)
+        if (reinterpret_cast<uintptr_t>(q) & 3) return true;
+    for (long x : strides)
+        if (x & 1) return true;
+    return false;
+}
+
 // Four columns a workgroup or 16, for at most four rows: 16 where the columns make a workgroup per compute unit anyway and four
 // would leave wavefronts without a piece of the reduction, if it is one turn, or a pair of filters to read (bf16, us, 4 / 16
 // columns: 1024 -> 4096 3.8 / 3.3, pair 2048 -> 8192 16.0 / 12.6; 2048 -> 8192 7.8 / 8.5, 4096 -> 4096 7.6 / 8.6, 8192 -> 512 4.7 / 10.6).
@@ -171,40 +195,45 @@ bool few_columns(const DenseFewRows &a)
     return !(filled && idle && (a.gated || a.K <= TURN));
 }
 
-template <typename T, bool GATED>
+template <typename T, bool ODD, bool GATED>
 hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
 {
     const dim3 block(FEW_WAVES * 64), grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 63) / 64));
-    if (a.M <= 4 && few_columns<T>(a)) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 1, 4>), dim3((unsigned)((a.N + 3) / 4)), block, 0, s, a);
-    else if (a.M <= 16) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 1, 16>), grid, block, 0, s, a);
-    else if (a.M <= 32) hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 2, 16>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((dense_few_rows_kernel<T, GATED, 4, 16>), grid, block, 0, s, a);
+    if (a.M <= 4 && few_columns<T>(a)) hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 1, 4>), dim3((unsigned)((a.N + 3) / 4)), block, 0, s, a);
+    else if (a.M <= 16) hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 1, 16>), grid, block, 0, s, a);
+    else if (a.M <= 32) hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 2, 16>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 4, 16>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 // Up to 16 rows always: W is the time, and this kernel reads it once and as it is. More rows: by an estimate against the tile
-// kernel's. A workgroup's turn (1024 k of bf16, 512 of fp32) of 2 / 4 blocks of rows takes 2.7 / 4.7 us in bf16, 2.7 / 6.5 in
-// fp32, 1.4 and 1.6 times that for a gated pair (measured on 512 x 1000 to 4096 x 4096 filters). E.g. 200 rows of 512 x 1000
+// kernel's, fitted to 20 .. 4096 rows of 64 x 64 to 4096 x 4096 filters (within 10 %). A workgroup with 2 / 4 blocks of rows
+// takes 0.9 / 1.7 us and 2.2 / 4.0 us a turn of 1024 k in bf16, 0.6 / 1.3 and 2.3 / 4.4 us a turn of 512 k in fp32, a gated pair
+// 1.35 and 1.55 times that; what does not fit on the device at once takes 1.25 times as long again. E.g. 200 rows of 512 x 1000
 // bf16: 5.4 us here, 9 to 18 through tiles; 128 rows of 4096 x 4096: 39 against 20.
 bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K)
 {
     if (M <= 16) return true;
     if ((M + 63) / 64 > 65535) return false;   // (the grid's second dimension)
-    static constexpr double turn_us[2][2] = {{2.7, 4.7}, {2.7, 6.5}};
-    const int cus = device_cu_count() > 0 ? device_cu_count() : 1;
-    const double groups = (double)((N + 15) / 16) * ((M + 63) / 64), turns = (double)K / (f32 ? 512 : 1024);
-    const double turn = turn_us[f32 ? 1 : 0][M > 32] * (!gated ? 1.0 : f32 ? 1.6 : 1.4);
-    const double us = 2.0 + (groups > cus ? groups / cus : 1.0) * (0.7 + (turns < 0.5 ? 0.5 : turns) * turn);
-    return us < dense_product_us(M, N, K, f32, 1, gated);
+    static constexpr double group_us[2][2] = {{0.9, 1.7}, {0.6, 1.3}}, turn_us[2][2] = {{2.2, 4.0}, {2.3, 4.4}};
+    const int cus = device_cu_count() > 0 ? device_cu_count() : 1, blocks = M > 32;
+    const double groups = (double)((N + 15) / 16) * ((M + 63) / 64), more = groups > cus ? groups / cus - 1.0 : 0.0;
+    const double turns = (double)K / (f32 ? 512 : 1024), group = group_us[f32 != 0][blocks] + (turns < 0.25 ? 0.25 : turns) * turn_us[f32 != 0][blocks];
+    const double us = 2.0 + group * (!gated ? 1.0 : f32 ? 1.55 : 1.35) * (1.0 + 1.25 * more);
+    // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
+    const double copies = !f32 && K % 8 ? 6.0 + ((double)M + N) * K * 4 / 4e6 : 0.0;
+    return us < dense_product_us(M, N, K, f32, 1, gated) + copies;
 }
 
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a)
 {
     if (a.M <= 0 || a.N <= 0) return hipSuccess;
-    if (a.gated) return a.f32 ? launch_few<float, true>(s, a) : launch_few<__bf16, true>(s, a);
-    return a.f32 ? launch_few<float, false>(s, a) : launch_few<__bf16, false>(s, a);
+    if (a.f32) return a.gated ? launch_few<float, false, true>(s, a) : launch_few<float, false, false>(s, a);
+    // (K: the last load of a row begins at K - 8)
+    if (odd_rows({a.X, a.W, a.W2}, {a.M > 1 ? a.ldX : 0, a.ldW, a.gated ? a.ldW2 : 0, a.K})) return a.gated ? launch_few<__bf16, true, true>(s, a) : launch_few<__bf16, true, false>(s, a);
+    return a.gated ? launch_few<__bf16, false, true>(s, a) : launch_few<__bf16, false, false>(s, a);
 }
 
 }  // namespace alpha

@@ -145,7 +145,9 @@ bool dense_small_preferred(int f32, int M, int N, int K, int sources)
     const long groups = ((long)M + SMALL_M - 1) / SMALL_M * ((N + SMALL_N - 1) / SMALL_N), rounds = (groups + cus - 1) / cus;
     const double all = (double)K * sources, us = 3.0 + rounds * (1.0 + (f32 ? all * 0.0125 : (double)(long)((all + 255) / 256) * 0.9));
     // (the loads at an edge take what lies before it)
-    return M >= 2 && N >= 4 && K >= 8 && (M + SMALL_M - 1) / SMALL_M <= 65535 && us < dense_product_us(M, N, K, f32, sources, 0);
+    // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
+    const double copies = !f32 && N % 8 ? 3.0 + all * N * 4 / 4e6 : 0.0;
+    return M >= 2 && N >= 4 && K >= 8 && (M + SMALL_M - 1) / SMALL_M <= 65535 && us < dense_product_us(M, N, K, f32, sources, 0) + copies;
 }
 
 hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
@@ -163,13 +165,9 @@ hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
     a.sources = p.sources;
     a.ep = p.ep;
     const dim3 grid((unsigned)((p.N + SMALL_N - 1) / SMALL_N), (unsigned)((p.M + SMALL_M - 1) / SMALL_M)), block(SMALL_WAVES * 64);
-    if (p.a_t) {
-        if (p.f32) hipLaunchKernelGGL((dense_small_kernel<float, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((dense_small_kernel<__bf16, true>), grid, block, 0, s, a);
-    } else {
-        if (p.f32) hipLaunchKernelGGL((dense_small_kernel<float, false>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((dense_small_kernel<__bf16, false>), grid, block, 0, s, a);
-    }
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a); };
+    if (p.a_t) launch(p.f32 ? dense_small_kernel<float, true> : dense_small_kernel<__bf16, true>);
+    else launch(p.f32 ? dense_small_kernel<float, false> : dense_small_kernel<__bf16, false>);
     return hipGetLastError();
 }
 
