@@ -44,17 +44,17 @@ __device__ __forceinline__ typename FewVec<T>::type few_load(const T *row, int k
     }
     return v;
 }
-// what was loaded at K - V instead of at k > K - V, moved to its place: zeros from K on
+// what was loaded at end - V instead of at k > end - V, moved to its place: zeros from K on
 template <typename T>
-__device__ __forceinline__ typename FewVec<T>::type few_at_edge(typename FewVec<T>::type x, int k, int K)
+__device__ __forceinline__ typename FewVec<T>::type few_at_edge(typename FewVec<T>::type x, int k, int end, int K)
 {
     constexpr int V = 16 / sizeof(T);
     T v[V];
 #pragma unroll
     for (int e = 0; e < V; e++) v[e] = x[e];
-    at_edge<V>(k, K, v);
+    at_edge<V>(k, end, v);
 #pragma unroll
-    for (int e = 0; e < V; e++) x[e] = v[e];
+    for (int e = 0; e < V; e++) x[e] = sizeof(T) == 4 || k + e < K ? v[e] : (T)0.f;
     return x;
 }
 
@@ -96,13 +96,14 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
 
     // Every workgroup starts at another place of the reduction: rows are often a power of two apart, and workgroups that
     // all read the same k at a time would all ask the same few channels of the memory.
+    // (bf16, rows that begin with a word: the last load of a row ends with the word of its last element)
+    const int end = sizeof(T) == 2 && !ODD ? (a.K + 1) & ~1 : a.K, last = end - V;
     const int turns = a.K < V ? 0 : (a.K + FEW_WAVES * SPAN - 1) / (FEW_WAVES * SPAN);
     int turn = turns > 0 ? (int)(blockIdx.x % turns) : 0;
     for (int t = 0; t < turns; t++) {
         const int k0 = (turn * FEW_WAVES + wave) * SPAN, k = k0 + l16 / C * PIECE;
         if (k0 < a.K) {
             vec vw[G][4], vx[MB][4];
-            const int last = a.K - V;      // >= 0
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int at = k + c * CHUNK + q * V;
@@ -120,9 +121,9 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
             for (int c = 0; c < 4; c++) {
                 if (edge) {
 #pragma unroll
-                    for (int g = 0; g < G; g++) vw[g][c] = few_at_edge<T>(vw[g][c], k + c * CHUNK + q * V, a.K);
+                    for (int g = 0; g < G; g++) vw[g][c] = few_at_edge<T>(vw[g][c], k + c * CHUNK + q * V, end, a.K);
 #pragma unroll
-                    for (int b = 0; b < MB; b++) vx[b][c] = few_at_edge<T>(vx[b][c], k + c * CHUNK + q * V, a.K);
+                    for (int b = 0; b < MB; b++) vx[b][c] = few_at_edge<T>(vx[b][c], k + c * CHUNK + q * V, end, a.K);
                 }
 #pragma unroll
                 for (int g = 0; g < G; g++)
@@ -221,7 +222,8 @@ bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K)
     const int cus = device_cu_count() > 0 ? device_cu_count() : 1, blocks = M > 32;
     const double groups = (double)((N + 15) / 16) * ((M + 63) / 64), more = groups > cus ? groups / cus - 1.0 : 0.0;
     const double turns = (double)K / (f32 ? 512 : 1024), group = group_us[f32 != 0][blocks] + (turns < 0.25 ? 0.25 : turns) * turn_us[f32 != 0][blocks];
-    const double us = 2.0 + group * (!gated ? 1.0 : f32 ? 1.55 : 1.35) * (1.0 + 1.25 * more);
+    const double odd = !f32 && K % 2 ? 1.6 : 1.0;      // (rows one behind the other then begin in the middle of a word)
+    const double us = 2.0 + group * odd * (!gated ? 1.0 : f32 ? 1.55 : 1.35) * (1.0 + 1.25 * more);
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
     const double copies = !f32 && K % 8 ? 6.0 + ((double)M + N) * K * 4 / 4e6 : 0.0;
     return us < dense_product_us(M, N, K, f32, 1, gated) + copies;
@@ -231,8 +233,7 @@ hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a)
 {
     if (a.M <= 0 || a.N <= 0) return hipSuccess;
     if (a.f32) return a.gated ? launch_few<float, false, true>(s, a) : launch_few<float, false, false>(s, a);
-    // (K: the last load of a row begins at K - 8)
-    if (odd_rows({a.X, a.W, a.W2}, {a.M > 1 ? a.ldX : 0, a.ldW, a.gated ? a.ldW2 : 0, a.K})) return a.gated ? launch_few<__bf16, true, true>(s, a) : launch_few<__bf16, true, false>(s, a);
+    if (odd_rows({a.X, a.W, a.W2}, {a.M > 1 ? a.ldX : 0, a.ldW, a.gated ? a.ldW2 : 0})) return a.gated ? launch_few<__bf16, true, true>(s, a) : launch_few<__bf16, true, false>(s, a);
     return a.gated ? launch_few<__bf16, false, true>(s, a) : launch_few<__bf16, false, false>(s, a);
 }
 
