@@ -157,7 +157,7 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
 {
     Scratch ws(base);
     ForwardRoom r{};
-    if (dense_few_rows_preferred(type == ALPHA_DENSE_F32, gated, N, OC, IC)) return r;   // operands as they are, no pieces
+    if (dense_forward_form(type == ALPHA_DENSE_F32, gated, N, OC, IC) != DENSE_TILES_FORM) return r;   // operands as they are, no pieces
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
     r.piece_bytes = dense_product_piece_bytes(N, OC, IC, type == ALPHA_DENSE_F32, 1, gated);
@@ -195,7 +195,8 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
 int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, int64_t ldX, const void *W, int64_t ldW, const void *W2, int64_t ldW2,
             const DenseEpilogue &ep, int N, int IC, int OC, void *workspace)
 {
-    if (dense_few_rows_preferred(type == ALPHA_DENSE_F32, gated, N, OC, IC)) {
+    const DenseForm form = dense_forward_form(type == ALPHA_DENSE_F32, gated, N, OC, IC);
+    if (form != DENSE_TILES_FORM) {
         DenseFewRows a{};
         a.X = X;
         a.ldX = ldX;
@@ -209,7 +210,7 @@ int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, i
         a.N = OC;
         a.K = IC;
         a.ep = ep;
-        return hip_status(launch_dense_few_rows(s, a), fn);
+        return hip_status(form == DENSE_FEW_ROWS ? launch_dense_few_rows(s, a) : launch_dense_short(s, a), fn);
     }
     const ForwardRoom room = forward_room(type, N, IC, OC, gated, workspace);
     DenseProduct p{};

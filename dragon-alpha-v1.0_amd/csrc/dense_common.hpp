@@ -8,6 +8,7 @@ namespace alpha {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 // ---- activations ---------------------------------------------------------------------------------------------------
 // exp(-z) from the hardware's 2^x: z log2(e) as a rounded product and its remainder, the remainder applied to first order;
@@ -160,7 +161,12 @@ struct DenseFewRows {
     DenseEpilogue ep;
 };
 
-bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K);
+// How a forward product is computed: by tiles, or straight from memory as few rows or as a short reduction.
+enum DenseForm { DENSE_TILES_FORM, DENSE_FEW_ROWS, DENSE_SHORT };
+DenseForm dense_forward_form(int f32, int gated, int M, int N, int K);
+double dense_few_rows_us(int f32, int gated, int M, int N, int K);   // estimates
+double dense_short_us(int f32, int gated, int M, int N, int K);
+hipError_t launch_dense_short(hipStream_t s, const DenseFewRows &a);
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);
 
 // Small products of a backward (B with k as its rows), operands as they are, no pieces (dense_small.hip).

@@ -10,7 +10,7 @@
 // reduction times four (only the products of equal pieces are read out): four times as many workgroups, each with a
 // quarter of the reduction's length in turns (1 x 8192 x 1024 of bf16: 11.4 -> 5.4 us).
 // Rows may begin at any element and K may be any number.
-#include "dense_finish.hpp"
+#include "dense_direct.hpp"
 
 namespace alpha {
 
@@ -18,59 +18,11 @@ namespace {
 
 constexpr int FEW_WAVES = 8;
 
-template <typename T> struct FewVec;
-template <> struct FewVec<float> { typedef floatx4 type; };
-template <> struct FewVec<__bf16> { typedef bf16x8 type; };
-
-// 16 bytes of a row from element k on, whatever its alignment. ODD: bf16 that may begin in the middle of a word, which the memory
-// pipe serves at a third of its rate (100 x 2001 x 500 28.0 -> 17.2 us); the words they lie in are loaded instead and shifted. (The
-// half word beside them is dropped: it shares its word, and so its page, with an element that is asked for.)
-template <bool ODD, typename T>
-__device__ __forceinline__ typename FewVec<T>::type few_load(const T *row, int k)
-{
-    typename FewVec<T>::type v;
-    if constexpr (ODD) {
-        const char *c = reinterpret_cast<const char *>(row + k);
-        const unsigned odd = (unsigned)reinterpret_cast<uintptr_t>(c) & 2;
-        c -= odd;
-        uint32_t w[5];
-        __builtin_memcpy(w, __builtin_assume_aligned(c, 4), 16);
-        __builtin_memcpy(w + 4, __builtin_assume_aligned(c + 12 + 2 * odd, 4), 4);
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], odd * 8);
-        __builtin_memcpy(&v, w, 16);
-    } else {
-        __builtin_memcpy(&v, row + k, 16);
-    }
-    return v;
-}
-// what was loaded at end - V instead of at k > end - V, moved to its place: zeros from K on
-template <typename T>
-__device__ __forceinline__ typename FewVec<T>::type few_at_edge(typename FewVec<T>::type x, int k, int end, int K)
-{
-    constexpr int V = 16 / sizeof(T);
-    T v[V];
-#pragma unroll
-    for (int e = 0; e < V; e++) v[e] = x[e];
-    at_edge<V>(k, end, v);
-#pragma unroll
-    for (int e = 0; e < V; e++) x[e] = sizeof(T) == 4 || k + e < K ? v[e] : (T)0.f;
-    return x;
-}
-
-__device__ __forceinline__ floatx4 few_multiply(bf16x8 w, bf16x8 x, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
-__device__ __forceinline__ floatx4 few_multiply(floatx4 w, floatx4 x, floatx4 c)
-{
-#pragma unroll
-    for (int s = 0; s < 4; s++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(w[s], x[s], c, 0, 0, 0);
-    return c;
-}
-
 }  // namespace
 
 // C: columns of a workgroup, 16, or 4 for at most four rows. MB: blocks of 16 rows.
 template <typename T, bool ODD, bool GATED, int MB, int C>
-__global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const DenseFewRows a)
+__global__ __launch_bounds__(FEW_WAVES * 64, !ODD && !GATED && MB == 4 ? 4 : 2) void dense_few_rows_kernel(const DenseFewRows a)
 {
     typedef typename FewVec<T>::type vec;
     constexpr int V = 16 / sizeof(T), CHUNK = 4 * V, GROUPS = 16 / C;         // k of a lane, of a wavefront's load of a row
@@ -121,9 +73,9 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
             for (int c = 0; c < 4; c++) {
                 if (edge) {
 #pragma unroll
-                    for (int g = 0; g < G; g++) vw[g][c] = few_at_edge<T>(vw[g][c], k + c * CHUNK + q * V, end, a.K);
+                    for (int g = 0; g < G; g++) vw[g][c] = few_at_edge<T, ODD>(vw[g][c], k + c * CHUNK + q * V, end, a.K);
 #pragma unroll
-                    for (int b = 0; b < MB; b++) vx[b][c] = few_at_edge<T>(vx[b][c], k + c * CHUNK + q * V, end, a.K);
+                    for (int b = 0; b < MB; b++) vx[b][c] = few_at_edge<T, ODD>(vx[b][c], k + c * CHUNK + q * V, end, a.K);
                 }
 #pragma unroll
                 for (int g = 0; g < G; g++)
@@ -175,16 +127,6 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void dense_few_rows_kernel(const De
 
 namespace {
 
-// May a load of bf16 from these rows begin in the middle of a word?
-bool odd_rows(std::initializer_list<const void *> p, std::initializer_list<long> strides)
-{
-    for (const void *q : p)
-        if (reinterpret_cast<uintptr_t>(q) & 3) return true;
-    for (long x : strides)
-        if (x & 1) return true;
-    return false;
-}
-
 // Four columns a workgroup or 16, for at most four rows: 16 where the columns make a workgroup per compute unit anyway and four
 // would leave wavefronts without a piece of the reduction, if it is one turn, or a pair of filters to read (bf16, us, 4 / 16
 // columns: 1024 -> 4096 3.8 / 3.3, pair 2048 -> 8192 16.0 / 12.6; 2048 -> 8192 7.8 / 8.5, 4096 -> 4096 7.6 / 8.6, 8192 -> 512 4.7 / 10.6).
@@ -209,24 +151,34 @@ hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
 
 }  // namespace
 
-// Up to 16 rows always: W is the time, and this kernel reads it once and as it is. More rows: by an estimate against the tile
-// kernel's, fitted to 20 .. 4096 rows of 64 x 64 to 4096 x 4096 filters (within 10 %). A workgroup with 2 / 4 blocks of rows
-// takes 0.9 / 1.7 us and 2.2 / 4.0 us a turn of 1024 k in bf16, 0.6 / 1.3 and 2.3 / 4.4 us a turn of 512 k in fp32, a gated pair
-// 1.35 and 1.55 times that; what does not fit on the device at once takes 1.25 times as long again. E.g. 200 rows of 512 x 1000
-// bf16: 5.4 us here, 9 to 18 through tiles; 128 rows of 4096 x 4096: 39 against 20.
-bool dense_few_rows_preferred(int f32, int gated, int M, int N, int K)
+// Estimate in us, fitted to 20 .. 4592 rows of 32 x 64 to 2000 x 4368 filters (within 10 % where it decides): 2 us, and per
+// workgroup with 2 / 4 blocks of rows 0.7 / 1.0 us and 1.6 / 3.5 us a turn of 1024 k in bf16, 0.7 / 1.3 and 1.9 / 4.15 us a turn of
+// 512 k in fp32; a gated pair 0.9 / 2.1 and 2.4 / 3.75, 1.0 / 2.65 and 3.7 / 6.65. What does not fit on the compute units at
+// once takes that times `more` again (two workgroups of less than 128 registers share one).
+double dense_few_rows_us(int f32, int gated, int M, int N, int K)
 {
-    if (M <= 16) return true;
-    if ((M + 63) / 64 > 65535) return false;   // (the grid's second dimension)
-    static constexpr double group_us[2][2] = {{0.9, 1.7}, {0.6, 1.3}}, turn_us[2][2] = {{2.2, 4.0}, {2.3, 4.4}};
-    const int cus = device_cu_count() > 0 ? device_cu_count() : 1, blocks = M > 32;
-    const double groups = (double)((N + 15) / 16) * ((M + 63) / 64), more = groups > cus ? groups / cus - 1.0 : 0.0;
-    const double turns = (double)K / (f32 ? 512 : 1024), group = group_us[f32 != 0][blocks] + (turns < 0.25 ? 0.25 : turns) * turn_us[f32 != 0][blocks];
+    if ((M + 63) / 64 > 65535) return 1e30;   // (the grid's second dimension)
+    static constexpr double group_us[2][2][2] = {{{0.7, 1.0}, {0.9, 2.1}}, {{0.7, 1.3}, {1.0, 2.65}}};
+    static constexpr double turn_us[2][2][2] = {{{1.6, 3.5}, {2.4, 3.75}}, {{1.9, 4.15}, {3.7, 6.65}}};
+    static constexpr double more[2][2][2] = {{{0.5, 0.85}, {0.5, 1.3}}, {{0.8, 0.9}, {0.85, 1.15}}};
+    const int t = f32 != 0, g = gated != 0, b = M > 32;
+    const long cus = device_cu_count() > 0 ? device_cu_count() : 1, groups = ((long)N + 15) / 16 * ((M + 63) / 64);
+    const double turns = (double)K / (f32 ? 512 : 1024), group = group_us[t][g][b] + (turns < 0.25 ? 0.25 : turns) * turn_us[t][g][b];
     const double odd = !f32 && K % 2 ? 1.6 : 1.0;      // (rows one behind the other then begin in the middle of a word)
-    const double us = 2.0 + group * odd * (!gated ? 1.0 : f32 ? 1.55 : 1.35) * (1.0 + 1.25 * more);
+    return 2.0 + group * odd * (1.0 + more[t][g][b] * (double)((groups + cus - 1) / cus - 1));
+}
+
+// Up to 16 rows always this kernel: W is the time, and it is read once and as it is. Else the least estimate. Measured, us, bf16
+// through (few rows / short / tiles): 384 x 96 x 4368 19 / 6.6 / 9.2, 384 x 1000 x 64 6.0 / 12 / 8.8, 1500 x 1000 x 320 9.9 /
+// 12.5 / 13.9; fp32 384 x 96 x 4368 20 / 13.8 / 16.7, 384 x 520 x 1344 12 / 17.8 / 20.9, 128 x 4096 x 4096 bf16 39 / - / 20.
+DenseForm dense_forward_form(int f32, int gated, int M, int N, int K)
+{
+    if (M <= 16) return DENSE_FEW_ROWS;
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
     const double copies = !f32 && K % 8 ? 6.0 + ((double)M + N) * K * 4 / 4e6 : 0.0;
-    return us < dense_product_us(M, N, K, f32, 1, gated) + copies;
+    const double few = dense_few_rows_us(f32, gated, M, N, K), brief = dense_short_us(f32, gated, M, N, K);
+    const double tiles = dense_product_us(M, N, K, f32, 1, gated) + copies;
+    return tiles <= few && tiles <= brief ? DENSE_TILES_FORM : few <= brief ? DENSE_FEW_ROWS : DENSE_SHORT;
 }
 
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a)

@@ -7,7 +7,6 @@
 
 namespace alpha {
 
-typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
