@@ -14,7 +14,7 @@ namespace alpha {
 
 namespace {
 
-constexpr int SMALL_WAVES = 8, SMALL_M = 32, SMALL_N = 64;
+constexpr int SMALL_WAVES = 8;
 
 }  // namespace
 
@@ -25,18 +25,20 @@ struct DenseSmallArgs {
     DenseEpilogue ep;
 };
 
-template <typename T, bool AT>
+// TM x TN: MFMA tiles of a workgroup, 2 x 4 or 1 x 2
+template <typename T, bool AT, int TM, int TN>
 __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const DenseSmallArgs a)
 {
+    constexpr int SMALL_M = 16 * TM, SMALL_N = 16 * TN;
     constexpr int CHUNK = sizeof(T) == 4 ? 16 : 32, V = CHUNK / 4;   // k of a chunk, of a lane
-    __shared__ floatx4 part[SMALL_WAVES][8][64];
+    __shared__ floatx4 part[SMALL_WAVES][TM * TN][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
     const int m0 = blockIdx.y * SMALL_M, n0 = blockIdx.x * SMALL_N;
-    floatx4 acc[2][4];
+    floatx4 acc[TM][TN];
 #pragma unroll
-    for (int t = 0; t < 2; t++)
+    for (int t = 0; t < TM; t++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[t][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TN; j++) acc[t][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
     const int chunks = (a.K + CHUNK - 1) / CHUNK;
     const bool edge_m = m0 + SMALL_M > a.M, edge_n = n0 + SMALL_N > a.N;
@@ -44,15 +46,15 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
         const bool second = c >= chunks;
         const T *A = static_cast<const T *>(second ? a.A[1] : a.A[0]), *B = static_cast<const T *>(second ? a.B[1] : a.B[0]);
         const int k0 = (second ? c - chunks : c) * CHUNK, k = k0 + q * V;     // the chunk's first, the lane's first
-        T b[V][4], x[2][V], xt[V][2];                                         // x[t]: A's tile t
+        T b[V][TN], x[TM][V], xt[V][TM];                                       // x[t]: A's tile t
 #pragma unroll
-        for (int s = 0; s < V; s++) load_columns<4>(B + (k + s < a.K ? k + s : a.K - 1) * a.ldB, n0 + 4 * l16, a.N, b[s]);
+        for (int s = 0; s < V; s++) load_columns<TN>(B + (k + s < a.K ? k + s : a.K - 1) * a.ldB, n0 + TN * l16, a.N, b[s]);
         if constexpr (AT) {
 #pragma unroll
-            for (int s = 0; s < V; s++) load_columns<2>(A + (k + s < a.K ? k + s : a.K - 1) * a.ldA, m0 + 2 * l16, a.M, xt[s]);
+            for (int s = 0; s < V; s++) load_columns<TM>(A + (k + s < a.K ? k + s : a.K - 1) * a.ldA, m0 + TM * l16, a.M, xt[s]);
         } else {
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < TM; t++) {
                 const int m = m0 + 16 * t + l16;
                 load_columns<V>(A + (m < a.M ? m : a.M - 1) * a.ldA, k, a.K, x[t]);
             }
@@ -60,94 +62,114 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
         // edges, each uniform; what lies beyond K must be zero in both operands, columns beyond C's edge are not stored
         if (edge_n) {
 #pragma unroll
-            for (int s = 0; s < V; s++) at_edge<4>(n0 + 4 * l16, a.N, b[s]);
+            for (int s = 0; s < V; s++) at_edge<TN>(n0 + TN * l16, a.N, b[s]);
         }
         if constexpr (AT) {
             if (edge_m) {
 #pragma unroll
-                for (int s = 0; s < V; s++) at_edge<2>(m0 + 2 * l16, a.M, xt[s]);
+                for (int s = 0; s < V; s++) at_edge<TM>(m0 + TM * l16, a.M, xt[s]);
             }
 #pragma unroll
-            for (int s = 0; s < V; s++) {
-                x[0][s] = xt[s][0];
-                x[1][s] = xt[s][1];
-            }
+            for (int s = 0; s < V; s++)
+#pragma unroll
+                for (int t = 0; t < TM; t++) x[t][s] = xt[s][t];
         }
         if (k0 + CHUNK > a.K) {
 #pragma unroll
             for (int s = 0; s < V; s++) {
                 const bool there = k + s < a.K;
 #pragma unroll
-                for (int j = 0; j < 4; j++) b[s][j] = there ? b[s][j] : (T)0.f;
+                for (int j = 0; j < TN; j++) b[s][j] = there ? b[s][j] : (T)0.f;
                 if constexpr (AT) {
-                    x[0][s] = there ? x[0][s] : (T)0.f;
-                    x[1][s] = there ? x[1][s] : (T)0.f;
+#pragma unroll
+                    for (int t = 0; t < TM; t++) x[t][s] = there ? x[t][s] : (T)0.f;
                 }
             }
             if constexpr (!AT) {
-                at_edge<V>(k, a.K, x[0]);
-                at_edge<V>(k, a.K, x[1]);
+#pragma unroll
+                for (int t = 0; t < TM; t++) at_edge<V>(k, a.K, x[t]);
             }
         }
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int s = 0; s < V; s++)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
+                for (int t = 0; t < TM; t++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[s][j], x[t][s], acc[t][j], 0, 0, 0);
+                    for (int j = 0; j < TN; j++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[s][j], x[t][s], acc[t][j], 0, 0, 0);
         } else {
-            bf16x8 fx[2];
+            bf16x8 fx[TM];
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < TM; t++)
 #pragma unroll
                 for (int s = 0; s < 8; s++) fx[t][s] = x[t][s % V];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < TN; j++) {
                 bf16x8 fb;
 #pragma unroll
                 for (int s = 0; s < 8; s++) fb[s] = b[s % V][j];
 #pragma unroll
-                for (int t = 0; t < 2; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fx[t], acc[t][j], 0, 0, 0);
+                for (int t = 0; t < TM; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fx[t], acc[t][j], 0, 0, 0);
             }
         }
     }
 #pragma unroll
-    for (int t = 0; t < 2; t++)
+    for (int t = 0; t < TM; t++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) part[wave][t * 4 + j][lane] = acc[t][j];
+        for (int j = 0; j < TN; j++) part[wave][t * TN + j][lane] = acc[t][j];
     __syncthreads();
-    // MFMA (t, j): lane (l16, q), element e: column i = 4 q + e of the MFMA, which is n0 + 4 i + j; row l16, which is m0 + 16 t +
-    // l16, or m0 + 2 l16 + t where A has k as its rows. A thread takes four consecutive columns of a row: one i, j = 0 .. 3.
+    // MFMA (t, j): lane (l16, q), element e: column i = 4 q + e of the MFMA, which is n0 + TN i + j; row l16, which is m0 + 16 t +
+    // l16, or m0 + TM l16 + t where A has k as its rows. A thread takes TN consecutive columns of a row: one i, j = 0 .. TN - 1.
     const int row = threadIdx.x >> 4, i = threadIdx.x & 15;
-    const int m = m0 + row, n = n0 + 4 * i;
-    if (m >= a.M || n >= a.N) return;
-    const int t = AT ? row & 1 : row >> 4, at = (i >> 2) * 16 + (AT ? row >> 1 : row & 15);
-    float v[4];
+    const int m = m0 + row, n = n0 + TN * i;
+    if (row >= SMALL_M || m >= a.M || n >= a.N) return;
+    const int t = AT ? row % TM : row >> 4, at = (i >> 2) * 16 + (AT ? row / TM : row & 15);
+    float v[TN];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < TN; j++) {
         v[j] = 0.f;
 #pragma unroll
-        for (int w = 0; w < SMALL_WAVES; w++) v[j] += reinterpret_cast<const float *>(&part[w][t * 4 + j][at])[i & 3];
+        for (int w = 0; w < SMALL_WAVES; w++) v[j] += reinterpret_cast<const float *>(&part[w][t * TN + j][at])[i & 3];
     }
-    if (a.ep.vec && n + 4 <= a.N) {
-        dense_finish<T, 4, false, true>(a.ep, v, m, n);
-    } else {
-        dense_finish<T, 4, false, false>(a.ep, v, m, n, a.N - n < 4 ? a.N - n : 4);
+    if constexpr (TN == 4) {
+        if (a.ep.vec && n + 4 <= a.N) {
+            dense_finish<T, 4, false, true>(a.ep, v, m, n);
+            return;
+        }
     }
+    dense_finish<T, TN, false, false>(a.ep, v, m, n, a.N - n < TN ? a.N - n : TN);
 }
 
-// By an estimate against the tile kernels': a workgroup's reduction takes 12.5 ns a k in fp32 (its MFMAs), 0.9 us a turn of 256 k
-// in bf16 (the loads). 100 x 2000 x 500 backward in fp32 / bf16: 14 + 14 / 13 + 8 us through tiles, 10 + 8 / 7 + 5 here.
+namespace {
+
+// The smaller tile where it is faster by the estimate, which is returned.
+struct SmallTiles {
+    bool few;
+    double us;
+};
+// Estimate in us, fitted to products of 16 .. 4400 x 32 .. 3000 x 32 .. 4400 (within 10 % in fp32, 20 % in bf16): a start, the
+// reduction by k (fp32: 4 / 7 ns with the smaller and larger tile) or turns of 128 (bf16: 0.33 / 0.57 us), and as much as that
+// again and an epilogue for every workgroup a compute unit. Measured, smaller / larger / tile kernels: 200 x 240 x 760 bf16 4.1 /
+// 6.0 / 10.0, fp32 5.9 / 11.6 / 14.1; 200 x 3000 x 1500 deltaW bf16 38 / 21 / 17.
+SmallTiles small_tiles(int f32, int M, int N, int K, int sources)
+{
+    const long cus = device_cu_count() > 0 ? device_cu_count() : 1, all = (long)K * sources;
+    const double length = f32 ? (double)all : (double)((all + 127) / 128);
+    auto per_cu = [&](int m, int n) { return (double)(((long)M + m - 1) / m * ((N + n - 1) / n)) / cus; };
+    const double few = f32 ? 2.25 + length * 0.004 + per_cu(16, 32) * (0.23 + length * 0.004) : 2.2 + length * 0.33 + per_cu(16, 32) * (0.06 + length * 0.37);
+    const double many = f32 ? 3.05 + length * 0.007 + per_cu(32, 64) * (1.2 + length * 0.011) : 2.8 + length * 0.57 + per_cu(32, 64) * (1.4 + length * 0.35);
+    return few < many ? SmallTiles{true, few} : SmallTiles{false, many};
+}
+
+}  // namespace
+
+// By the estimates.
 bool dense_small_preferred(int f32, int M, int N, int K, int sources)
 {
-    const int cus = device_cu_count() > 0 ? device_cu_count() : 1;
-    const long groups = ((long)M + SMALL_M - 1) / SMALL_M * ((N + SMALL_N - 1) / SMALL_N), rounds = (groups + cus - 1) / cus;
-    const double all = (double)K * sources, us = 3.0 + rounds * (1.0 + (f32 ? all * 0.0125 : (double)(long)((all + 255) / 256) * 0.9));
-    // (the loads at an edge take what lies before it)
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
-    const double copies = !f32 && N % 8 ? 3.0 + all * N * 4 / 4e6 : 0.0;
-    return M >= 2 && N >= 4 && K >= 8 && (M + SMALL_M - 1) / SMALL_M <= 65535 && us < dense_product_us(M, N, K, f32, sources, 0) + copies;
+    const double copies = !f32 && N % 8 ? 3.0 + (double)K * sources * N * 4 / 4e6 : 0.0;
+    // (the loads at an edge take what lies before it; the grid's second dimension)
+    return M >= 2 && N >= 4 && K >= 8 && (M + 15) / 16 <= 65535 && small_tiles(f32, M, N, K, sources).us < dense_product_us(M, N, K, f32, sources, 0) + copies;
 }
 
 hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
@@ -164,10 +186,17 @@ hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
     a.K = p.K;
     a.sources = p.sources;
     a.ep = p.ep;
-    const dim3 grid((unsigned)((p.N + SMALL_N - 1) / SMALL_N), (unsigned)((p.M + SMALL_M - 1) / SMALL_M)), block(SMALL_WAVES * 64);
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a); };
-    if (p.a_t) launch(p.f32 ? dense_small_kernel<float, true> : dense_small_kernel<__bf16, true>);
-    else launch(p.f32 ? dense_small_kernel<float, false> : dense_small_kernel<__bf16, false>);
+    auto launch = [&](auto kernel, int tm, int tn) {
+        const dim3 grid((unsigned)((p.N + 16 * tn - 1) / (16 * tn)), (unsigned)((p.M + 16 * tm - 1) / (16 * tm)));
+        hipLaunchKernelGGL(kernel, grid, dim3(SMALL_WAVES * 64), 0, s, a);
+    };
+    if (small_tiles(p.f32, p.M, p.N, p.K, p.sources).few) {
+        if (p.a_t) launch(p.f32 ? dense_small_kernel<float, true, 1, 2> : dense_small_kernel<__bf16, true, 1, 2>, 1, 2);
+        else launch(p.f32 ? dense_small_kernel<float, false, 1, 2> : dense_small_kernel<__bf16, false, 1, 2>, 1, 2);
+    } else {
+        if (p.a_t) launch(p.f32 ? dense_small_kernel<float, true, 2, 4> : dense_small_kernel<__bf16, true, 2, 4>, 2, 4);
+        else launch(p.f32 ? dense_small_kernel<float, false, 2, 4> : dense_small_kernel<__bf16, false, 2, 4>, 2, 4);
+    }
     return hipGetLastError();
 }
 
