@@ -45,22 +45,22 @@ struct Scratch {
     }
 };
 
-bool sizes_served(int type, int64_t N, int64_t IC, int64_t OC)
+bool sizes_served(int type, int64_t N, int64_t IC, int64_t OC, int pair = 1)
 {
     if (type != ALPHA_DENSE_F32 && type != ALPHA_DENSE_BF16) return false;
-    if (N < 0 || IC < 0 || OC < 0 || IC > (1 << 22) || OC > (1 << 22)) return false;
+    if (N < 0 || IC < 0 || OC < 0 || IC > (1 << 22) || pair * OC > (1 << 22)) return false;   // (a pair's deltaZ lie side by side)
     // packed tensors of at most 2^34 elements: their 16-byte chunks are counted in 31 bits
     return N * round8(IC) < (1l << 34) && 2 * N * round8(OC) < (1l << 34) && OC * round8(IC) < (1l << 34);
 }
 
 int check_call(const char *fn, const int64_t *streams, int length, int type, int N, int IC, int OC, int act, float k, const void *workspace,
-               int64_t bytes, int64_t need)
+               int64_t bytes, int64_t need)   // need < 0: sizes not served
 {
     if (streams == nullptr || length < 1) return fail("%s: empty stream array", fn);
     if (type != ALPHA_DENSE_F32 && type != ALPHA_DENSE_BF16) return fail("%s: unknown element type %d", fn, type);
     if (act < ALPHA_DENSE_ACT_NONE || act > ALPHA_DENSE_ACT_SIGMOID) return fail("%s: unknown activation %d", fn, act);
     if (act == ALPHA_DENSE_ACT_LEAKY_RELU && !std::isfinite(k)) return fail("%s: slope k is not finite", fn);
-    if (!sizes_served(type, N, IC, OC) || need < 0) return fail("%s: size out of range (N %d, IC %d, OC %d)", fn, N, IC, OC);
+    if (need < 0) return fail("%s: size out of range (N %d, IC %d, OC %d)", fn, N, IC, OC);
     if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) || bytes < need))
         return fail("%s: workspace is null, not 256-byte aligned or too small (%lld of %lld bytes)", fn, (long long)bytes, (long long)need);
     return 0;
@@ -420,7 +420,7 @@ ALPHA_EXPORT int alpha_dmatMul_fused(const int64_t *streams, int length, int typ
 
 ALPHA_EXPORT int64_t alpha_gatedMatMul_workspace(int type, int N, int IC, int OC)
 {
-    return sizes_served(type, N, IC, OC) ? (int64_t)forward_room(type, N, IC, OC, 1, nullptr).total : -1;
+    return sizes_served(type, N, IC, OC, 2) ? (int64_t)forward_room(type, N, IC, OC, 1, nullptr).total : -1;
 }
 
 ALPHA_EXPORT int alpha_gatedMatMul(const int64_t *streams, int length, int type, const void *X, int64_t X_stride, const void *Wg, int64_t Wg_stride,
@@ -460,7 +460,7 @@ ALPHA_EXPORT int alpha_gatedMatMul(const int64_t *streams, int length, int type,
 
 ALPHA_EXPORT int64_t alpha_dgatedMatMul_workspace(int type, int N, int IC, int OC)
 {
-    return sizes_served(type, N, IC, OC) ? (int64_t)backward_room(type, N, IC, OC, 1, nullptr).total : -1;
+    return sizes_served(type, N, IC, OC, 2) ? (int64_t)backward_room(type, N, IC, OC, 1, nullptr).total : -1;
 }
 
 ALPHA_EXPORT int alpha_dgatedMatMul(const int64_t *streams, int length, int type, const void *deltaH, int64_t deltaH_stride, const void *G,

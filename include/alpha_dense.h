@@ -9,8 +9,10 @@
  *     tensor). Sums are held in fp32 (the norm's in fp64) and rounded once, to the output's type; bf16 backward rounds
  *     deltaZ (deltaG, deltaU) to bf16 before its products, deltaB is summed from the unrounded values.
  *   - Matrices are row-major, X[N,IC], W[OC,IC] (a filter W[OC,1,1,IC]), Y[N,OC]; `*_stride` is the distance of two rows
- *     in elements (>= the row's length, <= 2^22). Any size, any stride, pointers aligned to their element; rows whose
- *     length and stride are multiples of 8 (bf16) or 4 (fp32) elements on 16-byte aligned pointers take the fastest path.
+ *     in elements (>= the row's length, <= 2^22). IC, OC <= 2^22 (OC of a gated pair <= 2^21), any other size, any stride,
+ *     pointers aligned to their element. Large bf16 products copy operands whose row length or stride is no multiple of 8
+ *     elements, or whose address is no multiple of 16 bytes, into the workspace; all others are read in place. A bf16
+ *     element is read with the 4-byte word it lies in.
  *   - N, IC and OC may be 0: an empty sum is 0 (IC = 0: Z = Bias; N = 0: deltaW and deltaB are zeros).
  *   - All pointers are DEVICE pointers, borrowed for the duration of the enqueued work. Nothing is allocated, freed or
  *     synchronised; scratch is supplied by the caller: alpha_*_workspace gives its bytes for a call's type and sizes (0 to 2^63-1,
@@ -20,8 +22,9 @@
  *   - `streams`, `length`: as in alpha_conv.h; everything is enqueued on streams[0], which belongs to the current device,
  *     as does the memory. Calls may be captured into a graph. Results are bit-identical from run to run.
  *   - Outputs must not overlap inputs, the workspace or each other, except where said.
- *   - fp32 products of more than a few rows run on the bf16 matrix pipe as sums of exact three-part splits (24 bits): six
- *     of the nine partial products, the left-out ones below 2^-23 of a product. Infinities and NaN come out as in plain fp32.
+ *   - Large fp32 products run on the bf16 matrix pipe as sums of exact three-part splits (24 bits): six of the nine partial
+ *     products, the left-out ones together below 2^-23 of a product. Others are plain fp32. Infinities and NaN come out as in
+ *     plain fp32 either way.
  *
  * Return value: 0 on success, a hipError_t value, or ALPHA_DENSE_EINVAL; alpha_dense_last_error() has the thread's message.
  */

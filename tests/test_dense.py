@@ -117,3 +117,13 @@ def test_gradClip_workspace():
     with pytest.raises(pkg.AlphaConvError):
         D.gradClip_workspace(1, [-1])
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_a_pair_of_filters_has_half_the_columns():
+    # their deltaZ lie side by side in one row, whose length has the limit of a stride
+    for code in (D.F32, D.BF16):
+        assert D.gatedMatMul_workspace(code, 8, 8, 1 << 21) >= 0 and D.dgatedMatMul_workspace(code, 8, 8, 1 << 21) > 0
+        assert D.matMul_fused_workspace(code, 8, 8, 1 << 22) >= 0 and D.dmatMul_fused_workspace(code, 8, 8, 1 << 22) > 0
+        for query in (D.gatedMatMul_workspace, D.dgatedMatMul_workspace):
+            with pytest.raises(pkg.AlphaConvError):
+                query(code, 8, 8, (1 << 21) + 1)

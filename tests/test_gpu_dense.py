@@ -703,3 +703,32 @@ def test_in_place_residual_and_numpy_oracle():
                    5, 12, 6, ws.data_ptr(), n)
     torch.cuda.synchronize()
     assert np.allclose(y.cpu().numpy(), want, rtol=1e-5, atol=1e-5)
+
+
+# ---- reductions and edges of the forms that read their operands straight from memory --------------------------------
+DIRECT = [(100, 2001, 70), (40, 1023, 33), (384, 9, 200), (384, 33, 777), (130, 96, 1000), (700, 41, 130), (2000, 129, 70), (257, 255, 65), (90, 15, 500)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("size", DIRECT)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (1, 0), (0, 1), (3, 2), (2, 3)])
+def test_forward_of_short_reductions_and_odd_rows(kind, size, pad, offset):
+    check_forward(kind, *size, act=D.ACT_LEAKY_RELU, residual=True, save=True, pad=pad, offset=offset)
+    check_gated(kind, *size, pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [2, 4, 5, 16])
+@pytest.mark.parametrize("ic,oc", [(7, 9), (8, 64), (9, 130), (2049, 61), (4097, 5000), (1000, 4100)])
+def test_few_rows_of_odd_lengths(kind, n, ic, oc):
+    check_forward(kind, n, ic, oc, act=D.ACT_SILU, residual=True, save=True, pad=1)
+    check_gated(kind, n, ic, oc)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("size", [(16, 36, 40), (200, 32, 760), (64, 70, 33), (1457, 64, 723), (33, 300, 9), (9, 5, 1500), (640, 333, 47)])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (1, 1), (3, 2)])
+def test_backward_of_small_products(kind, size, pad, offset):
+    check_backward(kind, *size, D.ACT_SILU, pad=pad, offset=offset)
+    check_backward(kind, *size, D.ACT_NONE, want=("dx", "dw"), pad=pad, offset=offset)
+    check_gated_backward(kind, *size, pad=pad, offset=offset)
