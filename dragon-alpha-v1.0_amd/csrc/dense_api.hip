@@ -293,7 +293,7 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
         p.ep.Y = c.dX;
         p.ep.ldY = c.ld_dX;
         p.ep.vec = quads_aligned(type, {c.dX}, {c.ld_dX});
-        const bool small = dense_small_preferred(p.f32, p.M, p.N, p.K, p.sources);
+        const bool small = dense_small_preferred(p.f32, 0, p.M, p.N, p.K, p.sources);
         if (OC > 0) {
             const bool strides = gated && c.ldW[0] != c.ldW[1];
             const bool pack = strides || (!small && (!in_place(type, c.W[0], c.ldW[0], IC) || (gated && !in_place(type, c.W[1], c.ldW[1], IC))));
@@ -323,7 +323,7 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
             p.ep.ldY2 = c.ld_dW[1];
             p.ep.vec = p.ep.vec && quads_aligned(type, {c.dW[1]}, {c.ld_dW[1]});
         }
-        const bool small = dense_small_preferred(p.f32, p.M, p.N, p.K, 1);
+        const bool small = dense_small_preferred(p.f32, 1, p.M, p.N, p.K, 1);
         if (N > 0) TRY(operand(fn, s, type, c.X, c.ldX, N, IC, room.X, !small && !in_place(type, c.X, c.ldX, IC), p.B, 0));
         TRY(hip_status(small ? launch_dense_small(s, p) : launch_dense_product(s, p), fn));
     }

@@ -138,35 +138,37 @@ bool few_columns(const DenseFewRows &a)
     return !(filled && idle && (a.gated || a.K <= TURN));
 }
 
-template <typename T, bool ODD, bool GATED>
-hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
-{
-    const dim3 block(FEW_WAVES * 64), grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 63) / 64));
-    if (a.M <= 4 && few_columns<T>(a)) hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 1, 4>), dim3((unsigned)((a.N + 3) / 4)), block, 0, s, a);
-    else if (a.M <= 16) hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 1, 16>), grid, block, 0, s, a);
-    else if (a.M <= 32) hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 2, 16>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((dense_few_rows_kernel<T, ODD, GATED, 4, 16>), grid, block, 0, s, a);
-    return hipGetLastError();
-}
-
 }  // namespace
 
-// Estimate in us, fitted to 20 .. 4592 rows of 32 x 64 to 2000 x 4368 filters (within 10 % where it decides): 2 us, and per
-// workgroup with 2 / 4 blocks of rows 0.7 / 1.0 us and 1.6 / 3.5 us a turn of 1024 k in bf16, 0.7 / 1.3 and 1.9 / 4.15 us a turn of
-// 512 k in fp32; a gated pair 0.9 / 2.1 and 2.4 / 3.75, 1.0 / 2.65 and 3.7 / 6.65. What does not fit on the compute units at
-// once takes that times `more` again (two workgroups of less than 128 registers share one).
-double dense_few_rows_us(int f32, int gated, int M, int N, int K)
+// Blocks of rows a workgroup, and the estimate in us that they are the least of, fitted to 17 .. 1500 rows of 64 x 64 to 4400 x 4368
+// filters (within 10 % where it decides): 2 us, and per workgroup with 1, 2, 4 blocks the times below, once and for each turn of
+// 1024 k in bf16, 512 k in fp32; what does not fit on the compute units at once takes that times `more` again (two workgroups of
+// at most 128 registers share one). Fewer blocks read W more often and use more compute units: 64 rows of 2000 x 296 take
+// 7.6 / 10.5 / 17.6 us in fp32 with 1 / 2 / 4 blocks, 5.0 / 6.4 / 9.4 in bf16.
+struct FewBlocks {
+    int blocks;      // of 16 rows a workgroup: 1, 2 or 4
+    double us;
+};
+static FewBlocks few_blocks(int f32, int gated, int M, int N, int K)
 {
-    if ((M + 63) / 64 > 65535) return 1e30;   // (the grid's second dimension)
-    static constexpr double group_us[2][2][2] = {{{0.7, 1.0}, {0.9, 2.1}}, {{0.7, 1.3}, {1.0, 2.65}}};
-    static constexpr double turn_us[2][2][2] = {{{1.6, 3.5}, {2.4, 3.75}}, {{1.9, 4.15}, {3.7, 6.65}}};
-    static constexpr double more[2][2][2] = {{{0.5, 0.85}, {0.5, 1.3}}, {{0.8, 0.9}, {0.85, 1.15}}};
-    const int t = f32 != 0, g = gated != 0, b = M > 32;
-    const long cus = device_cu_count() > 0 ? device_cu_count() : 1, groups = ((long)N + 15) / 16 * ((M + 63) / 64);
-    const double turns = (double)K / (f32 ? 512 : 1024), group = group_us[t][g][b] + (turns < 0.25 ? 0.25 : turns) * turn_us[t][g][b];
+    static constexpr double group_us[2][2][3] = {{{0.35, 0.6, 1.1}, {0.5, 1.0, 1.9}}, {{0.25, 0.5, 0.65}, {0.4, 0.9, 1.75}}};
+    static constexpr double turn_us[2][2][3] = {{{1.4, 1.9, 2.65}, {2.2, 2.65, 3.2}}, {{1.45, 2.2, 4.8}, {2.5, 4.1, 7.4}}};
+    static constexpr double more[2][2][3] = {{{0.7, 0.75, 0.9}, {0.85, 0.9, 1.45}}, {{0.8, 0.9, 0.9}, {0.95, 0.95, 1.2}}};
+    const int t = f32 != 0, g = gated != 0;
+    const long cus = device_cu_count() > 0 ? device_cu_count() : 1;
+    const double turns = (double)K / (f32 ? 512 : 1024);
     const double odd = !f32 && K % 2 ? 1.6 : 1.0;      // (rows one behind the other then begin in the middle of a word)
-    return 2.0 + group * odd * (1.0 + more[t][g][b] * (double)((groups + cus - 1) / cus - 1));
+    FewBlocks best{4, 1e30};
+    for (int b = 2; b >= 0; b--) {
+        const long rows = (M + (16l << b) - 1) / (16l << b), groups = ((long)N + 15) / 16 * rows;
+        if (rows > 65535) continue;   // (the grid's second dimension)
+        const double group = group_us[t][g][b] + (turns < 0.25 ? 0.25 : turns) * turn_us[t][g][b];
+        const double us = 2.0 + group * odd * (1.0 + more[t][g][b] * (double)((groups + cus - 1) / cus - 1));
+        if (us < best.us) best = FewBlocks{1 << b, us};
+    }
+    return best;
 }
+double dense_few_rows_us(int f32, int gated, int M, int N, int K) { return few_blocks(f32, gated, M, N, K).us; }
 
 // Up to 16 rows always this kernel: W is the time, and it is read once and as it is. Else the least estimate. Measured, us, bf16
 // through (few rows / short / tiles): 384 x 96 x 4368 19 / 6.6 / 9.2, 384 x 1000 x 64 6.0 / 12 / 8.8, 1500 x 1000 x 320 9.9 /
@@ -180,6 +182,28 @@ DenseForm dense_forward_form(int f32, int gated, int M, int N, int K)
     const double tiles = dense_product_us(M, N, K, f32, 1, gated) + copies;
     return tiles <= few && tiles <= brief ? DENSE_TILES_FORM : few <= brief ? DENSE_FEW_ROWS : DENSE_SHORT;
 }
+
+namespace {
+
+template <typename T, bool ODD, bool GATED>
+hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
+{
+    const dim3 block(FEW_WAVES * 64);
+    auto launch = [&](auto kernel, int columns, int rows) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.N + columns - 1) / columns), (unsigned)((a.M + rows - 1) / rows)), block, 0, s, a);
+    };
+    if (a.M <= 4 && few_columns<T>(a)) {
+        launch(dense_few_rows_kernel<T, ODD, GATED, 1, 4>, 4, 16);
+    } else {
+        const int blocks = a.M <= 16 ? 1 : few_blocks(sizeof(T) == 4, GATED, a.M, a.N, a.K).blocks;
+        if (blocks == 1) launch(dense_few_rows_kernel<T, ODD, GATED, 1, 16>, 16, 16);
+        else if (blocks == 2) launch(dense_few_rows_kernel<T, ODD, GATED, 2, 16>, 16, 32);
+        else launch(dense_few_rows_kernel<T, ODD, GATED, 4, 16>, 16, 64);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a)
 {

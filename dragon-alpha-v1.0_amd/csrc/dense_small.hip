@@ -163,13 +163,14 @@ SmallTiles small_tiles(int f32, int M, int N, int K, int sources)
 
 }  // namespace
 
-// By the estimates.
-bool dense_small_preferred(int f32, int M, int N, int K, int sources)
+// By the estimates. (A load at an edge takes what lies before it, so rows have at least one load: of columns of B, and of columns or
+// k of A.)
+bool dense_small_preferred(int f32, int a_t, int M, int N, int K, int sources)
 {
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
     const double copies = !f32 && N % 8 ? 3.0 + (double)K * sources * N * 4 / 4e6 : 0.0;
-    // (the loads at an edge take what lies before it; the grid's second dimension)
-    return M >= 2 && N >= 4 && K >= 8 && (M + 15) / 16 <= 65535 && small_tiles(f32, M, N, K, sources).us < dense_product_us(M, N, K, f32, sources, 0) + copies;
+    if (N < 4 || K < 1 || (a_t ? M < 2 : K < 8) || (M + 15) / 16 > 65535) return false;   // (65535: the grid's second dimension)
+    return small_tiles(f32, M, N, K, sources).us < dense_product_us(M, N, K, f32, sources, 0) + copies;
 }
 
 hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
