@@ -732,3 +732,11 @@ def test_backward_of_small_products(kind, size, pad, offset):
     check_backward(kind, *size, D.ACT_SILU, pad=pad, offset=offset)
     check_backward(kind, *size, D.ACT_NONE, want=("dx", "dw"), pad=pad, offset=offset)
     check_gated_backward(kind, *size, pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [1, 2, 3, 7])
+@pytest.mark.parametrize("ic,oc", [(4, 8), (5, 2), (64, 1728), (1217, 895), (784, 176)])
+def test_backward_of_few_rows(kind, n, ic, oc):
+    check_backward(kind, n, ic, oc, D.ACT_LEAKY_RELU, pad=1)
+    check_gated_backward(kind, n, ic, oc, pad=3)
