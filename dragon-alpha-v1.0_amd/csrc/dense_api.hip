@@ -181,11 +181,12 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < pair; i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
     r.sums = ws.take<float>(dense_delta_sum_bytes(N, OC, gated));
-    const size_t for_x = dense_product_piece_bytes(N, IC, OC, type == ALPHA_DENSE_F32, pair, 0);
+    auto pieces = [&](int a_t, int M, int N, int K, int sources) {
+        const int f32 = type == ALPHA_DENSE_F32;
+        return dense_small_preferred(f32, a_t, M, N, K, sources) ? dense_small_piece_bytes(f32, M, N, K, sources) : dense_product_piece_bytes(M, N, K, f32, sources, 0);
+    };
     // a gated pair's filter gradients are one stacked product, or one of them alone
-    const size_t for_w = std::max(dense_product_piece_bytes(OC, IC, N, type == ALPHA_DENSE_F32, 1, 0),
-                                  gated ? dense_product_piece_bytes((int)round8(OC) + OC, IC, N, type == ALPHA_DENSE_F32, 1, 0) : (size_t)0);
-    r.piece_bytes = std::max(for_x, for_w);
+    r.piece_bytes = std::max({pieces(0, N, IC, OC, pair), pieces(1, OC, IC, N, 1), gated ? pieces(1, (int)round8(OC) + OC, IC, N, 1) : (size_t)0});
     r.pieces = ws.take<float>(r.piece_bytes);
     r.total = ws.at;
     return r;

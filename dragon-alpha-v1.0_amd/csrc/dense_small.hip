@@ -10,6 +10,8 @@
 // Rows beyond K are zeros, rows and columns of C beyond its edge are not stored (their loads stay inside the operand).
 #include "dense_finish.hpp"
 
+#include <algorithm>
+
 namespace alpha {
 
 namespace {
@@ -22,6 +24,8 @@ struct DenseSmallArgs {
     const void *A[2], *B[2];
     long ldA, ldB;
     int M, N, K, sources;
+    int per;              // chunks of a workgroup
+    float *pieces;        // where the reduction is cut: [gridDim.z][M][columns, a multiple of 4]
     DenseEpilogue ep;
 };
 
@@ -42,7 +46,8 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
 
     const int chunks = (a.K + CHUNK - 1) / CHUNK;
     const bool edge_m = m0 + SMALL_M > a.M, edge_n = n0 + SMALL_N > a.N;
-    for (int c = wave; c < chunks * a.sources; c += SMALL_WAVES) {
+    const int all = chunks * a.sources, from = blockIdx.z * a.per, to = from + a.per < all ? from + a.per : all;
+    for (int c = from + wave; c < to; c += SMALL_WAVES) {
         const bool second = c >= chunks;
         const T *A = static_cast<const T *>(second ? a.A[1] : a.A[0]), *B = static_cast<const T *>(second ? a.B[1] : a.B[0]);
         const int k0 = (second ? c - chunks : c) * CHUNK, k = k0 + q * V;     // the chunk's first, the lane's first
@@ -131,6 +136,14 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
 #pragma unroll
         for (int w = 0; w < SMALL_WAVES; w++) v[j] += reinterpret_cast<const float *>(&part[w][t * TN + j][at])[i & 3];
     }
+    if (gridDim.z > 1) {
+        const long columns = (a.N + 3) & ~3;
+        float *to = a.pieces + ((long)blockIdx.z * a.M + m) * columns + n;
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+            if (n + j < columns) to[j] = v[j];
+        return;
+    }
     if constexpr (TN == 4) {
         if (a.ep.vec && n + 4 <= a.N) {
             dense_finish<T, 4, false, true>(a.ep, v, m, n);
@@ -140,28 +153,66 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void dense_small_kernel(const Den
     dense_finish<T, TN, false, false>(a.ep, v, m, n, a.N - n < TN ? a.N - n : TN);
 }
 
+// Adds the pieces of a cut reduction in their order: four columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_small_sum_kernel(const DenseSmallArgs a, int pieces, long quads, FastDiv d_quads)
+{
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads) return;
+    const long m = fdiv((uint32_t)i, d_quads), columns = (a.N + 3) & ~3;
+    const int n = (int)(i - m * d_quads.d) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < pieces; p++) {
+        const floatx4 t = quad_load(a.pieces + ((long)p * a.M + m) * columns + n);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += t[e];
+    }
+    if (a.ep.vec && n + 4 <= a.N) dense_finish<T, 4, false, true>(a.ep, v, m, n);
+    else dense_finish<T, 4, false, false>(a.ep, v, m, n, a.N - n < 4 ? a.N - n : 4);
+}
+
 namespace {
 
-// The smaller tile where it is faster by the estimate, which is returned.
-struct SmallTiles {
-    bool few;
+// Tile and cut of the reduction with the least estimate, which is in us.
+struct SmallPlan {
+    bool few;        // the smaller tile
+    int pieces, per; // per: chunks
     double us;
 };
-// Estimate in us, fitted to products of 16 .. 4400 x 32 .. 3000 x 32 .. 4400 (within 10 % in fp32, 20 % in bf16): a start, the
-// reduction by k (fp32: 4 / 7 ns with the smaller and larger tile) or turns of 128 (bf16: 0.33 / 0.57 us), and as much as that
-// again and an epilogue for every workgroup a compute unit. Measured, smaller / larger / tile kernels: 200 x 240 x 760 bf16 4.1 /
-// 6.0 / 10.0, fp32 5.9 / 11.6 / 14.1; 200 x 3000 x 1500 deltaW bf16 38 / 21 / 17.
-SmallTiles small_tiles(int f32, int M, int N, int K, int sources)
+// Estimate, fitted to products of 16 .. 4400 x 32 .. 3000 x 32 .. 4400 (within 10 % in fp32, 20 % in bf16): a start, the reduction by
+// k (fp32: 4 / 7 ns with the smaller and larger tile) or turns of 128 (bf16: 0.33 / 0.57 us), and as much as that again and an
+// epilogue for every workgroup a compute unit; a cut costs a second launch and the pieces' way through memory. Measured, smaller
+// / larger / tile kernels: 200 x 240 x 760 bf16 4.1 / 6.0 / 10.0, fp32 5.8 / 11.6 / 12.5; 200 x 3000 x 1500 deltaW bf16 38 / 21 /
+// 17; 64 x 320 of two reductions of 3136 fp32, in one piece and cut: 36.5 / 14.5.
+SmallPlan small_plan(int f32, int M, int N, int K, int sources)
 {
-    const long cus = device_cu_count() > 0 ? device_cu_count() : 1, all = (long)K * sources;
-    const double length = f32 ? (double)all : (double)((all + 127) / 128);
-    auto per_cu = [&](int m, int n) { return (double)(((long)M + m - 1) / m * ((N + n - 1) / n)) / cus; };
-    const double few = f32 ? 2.25 + length * 0.004 + per_cu(16, 32) * (0.23 + length * 0.004) : 2.2 + length * 0.33 + per_cu(16, 32) * (0.06 + length * 0.37);
-    const double many = f32 ? 3.05 + length * 0.007 + per_cu(32, 64) * (1.2 + length * 0.011) : 2.8 + length * 0.57 + per_cu(32, 64) * (1.4 + length * 0.35);
-    return few < many ? SmallTiles{true, few} : SmallTiles{false, many};
+    const long cus = device_cu_count() > 0 ? device_cu_count() : 1;
+    const int size = f32 ? 16 : 32, chunks = (K + size - 1) / size * sources;
+    SmallPlan best{false, 1, std::max(1, chunks), 1e30};
+    for (int few = 0; few < 2; few++) {
+        const long groups = few ? ((long)M + 15) / 16 * ((N + 31) / 32) : ((long)M + 31) / 32 * ((N + 63) / 64);
+        for (int pieces = 1; pieces <= 16; pieces *= 2) {
+            // (every piece of at least two turns of the eight wavefronts)
+            const int per = (chunks + pieces - 1) / pieces;
+            if (pieces > 1 && (groups * pieces > cus || per < 16 || (chunks + per - 1) / per != pieces)) break;
+            const double length = f32 ? per * 16.0 : (double)((per + 3) / 4), per_cu = (double)groups * pieces / cus;
+            double us = f32 ? (few ? 2.25 + length * 0.004 + per_cu * (0.23 + length * 0.004) : 3.05 + length * 0.007 + per_cu * (1.2 + length * 0.011))
+                            : (few ? 2.2 + length * 0.33 + per_cu * (0.06 + length * 0.37) : 2.8 + length * 0.57 + per_cu * (1.4 + length * 0.35));
+            if (pieces > 1) us += 2.5 + (double)pieces * M * N * 8 / 4.2e6;
+            if (us < best.us) best = SmallPlan{few != 0, pieces, per, us};
+        }
+    }
+    return best;
 }
 
 }  // namespace
+
+size_t dense_small_piece_bytes(int f32, int M, int N, int K, int sources)
+{
+    const SmallPlan plan = small_plan(f32, M, N, K, sources);
+    return plan.pieces > 1 ? (size_t)plan.pieces * M * ((N + 3) & ~3) * 4 : 0;
+}
 
 // By the estimates. (A load at an edge takes what lies before it, so rows have at least one load: of columns of B, and of columns or
 // k of A.)
@@ -170,11 +221,13 @@ bool dense_small_preferred(int f32, int a_t, int M, int N, int K, int sources)
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
     const double copies = !f32 && N % 8 ? 3.0 + (double)K * sources * N * 4 / 4e6 : 0.0;
     if (N < 4 || K < 1 || (a_t ? M < 2 : K < 8) || (M + 15) / 16 > 65535) return false;   // (65535: the grid's second dimension)
-    return small_tiles(f32, M, N, K, sources).us < dense_product_us(M, N, K, f32, sources, 0) + copies;
+    return small_plan(f32, M, N, K, sources).us < dense_product_us(M, N, K, f32, sources, 0) + copies;
 }
 
 hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
 {
+    const SmallPlan plan = small_plan(p.f32, p.M, p.N, p.K, p.sources);
+    if (plan.pieces > 1 && (p.pieces == nullptr || p.piece_bytes < dense_small_piece_bytes(p.f32, p.M, p.N, p.K, p.sources))) return hipErrorInvalidValue;
     DenseSmallArgs a{};
     for (int i = 0; i < 2; i++) {
         a.A[i] = p.A.p[i];
@@ -187,16 +240,25 @@ hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)
     a.K = p.K;
     a.sources = p.sources;
     a.ep = p.ep;
+    a.per = plan.per;
+    a.pieces = p.pieces;
     auto launch = [&](auto kernel, int tm, int tn) {
-        const dim3 grid((unsigned)((p.N + 16 * tn - 1) / (16 * tn)), (unsigned)((p.M + 16 * tm - 1) / (16 * tm)));
+        const dim3 grid((unsigned)((p.N + 16 * tn - 1) / (16 * tn)), (unsigned)((p.M + 16 * tm - 1) / (16 * tm)), (unsigned)plan.pieces);
         hipLaunchKernelGGL(kernel, grid, dim3(SMALL_WAVES * 64), 0, s, a);
     };
-    if (small_tiles(p.f32, p.M, p.N, p.K, p.sources).few) {
+    if (plan.few) {
         if (p.a_t) launch(p.f32 ? dense_small_kernel<float, true, 1, 2> : dense_small_kernel<__bf16, true, 1, 2>, 1, 2);
         else launch(p.f32 ? dense_small_kernel<float, false, 1, 2> : dense_small_kernel<__bf16, false, 1, 2>, 1, 2);
     } else {
         if (p.a_t) launch(p.f32 ? dense_small_kernel<float, true, 2, 4> : dense_small_kernel<__bf16, true, 2, 4>, 2, 4);
         else launch(p.f32 ? dense_small_kernel<float, false, 2, 4> : dense_small_kernel<__bf16, false, 2, 4>, 2, 4);
+    }
+    if (plan.pieces > 1) {   // (few workgroups, so few elements: their quads are counted in 31 bits)
+        const long row = (p.N + 3) / 4, quads = (long)p.M * row;
+        const FastDiv d = make_fastdiv((uint32_t)row);
+        const dim3 grid((unsigned)((quads + 255) / 256));
+        if (p.f32) hipLaunchKernelGGL((dense_small_sum_kernel<float>), grid, dim3(256), 0, s, a, plan.pieces, quads, d);
+        else hipLaunchKernelGGL((dense_small_sum_kernel<__bf16>), grid, dim3(256), 0, s, a, plan.pieces, quads, d);
     }
     return hipGetLastError();
 }

@@ -740,3 +740,11 @@ def test_backward_of_small_products(kind, size, pad, offset):
 def test_backward_of_few_rows(kind, n, ic, oc):
     check_backward(kind, n, ic, oc, D.ACT_LEAKY_RELU, pad=1)
     check_gated_backward(kind, n, ic, oc, pad=3)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,ic,oc", [(64, 320, 3136), (4416, 32, 34), (4416, 33, 35), (60, 100, 5001), (2, 5, 4099), (30000, 4, 6)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_backward_of_long_sums_of_few_results(kind, n, ic, oc, pad):
+    check_backward(kind, n, ic, oc, D.ACT_SIGMOID, pad=pad)
+    check_gated_backward(kind, n, ic, oc, pad=pad)
