@@ -1,7 +1,8 @@
 // The dense product for few rows of X or little work: no copy of an operand, one launch, as many bytes in flight as the
-// device takes. A single row reads W once and is bound by that.
+// device takes. A single row reads W once and is bound by that: 1 x 4096 x 4096 bf16 8.1 us, 4.2 TB/s; a gated pair 1 x 2048 x 8192
+// 12.4 us, 5.4 TB/s. More rows are bound by what a compute unit loads (35 to 40 bytes a nanosecond, whatever is in flight).
 //
-// A workgroup of eight wavefronts computes 16 columns of the output (16 rows of W) for up to 64 rows of X; its wavefronts
+// A workgroup of eight wavefronts computes 16 columns of the output (16 rows of W) for 16, 32 or 64 rows of X; its wavefronts
 // share the reduction in pieces of 256 bytes of every row. Both operands go straight from memory into the MFMA registers: a
 // lane holds 16 bytes of one row of W and of one row of X at the same k. bf16: v_mfma_f32_16x16x32_bf16, eight k a lane;
 // fp32: v_mfma_f32_16x16x4_f32, component s of the lane's four k in the s-th MFMA - plain fp32 products. Rows of X beyond

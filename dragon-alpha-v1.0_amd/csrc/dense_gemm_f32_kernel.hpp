@@ -2,7 +2,8 @@
 // the fp32 one. x = h + m + l exactly, three bf16 of 8 significant bits each (rounded to nearest, signs of their own); of the
 // nine products of parts the six above 2^-24 of the whole are summed, small ones first, in fp32:
 //     x y = h l' + m m' + h m' + l h' + m h' + h h'   (left out: m l', l m', l l', together below 2^-23 |x y|).
-// 2.5 PF / 6 = 417 TF bound, 157 TF through v_mfma_f32_16x16x4_f32.
+// 2.5 PF / 6 = 417 TF bound, 157 TF through v_mfma_f32_16x16x4_f32. Measured: 4096 x 1024 x 4096 with GELU and both outputs 178 us,
+// 193 TF; the matrix pipe is busy 54 % of the cycles at 1.84 GHz, the rest is the splitting, which it waits for.
 //
 // A workgroup takes BM x BN of C in steps of 32 k. An element is split once per workgroup: loaded to registers (128-bit buffer
 // loads, a step ahead), split, and written to LDS as three bf16 planes of the layout that dense_gemm_kernel.hpp describes, in

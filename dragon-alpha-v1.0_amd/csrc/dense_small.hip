@@ -1,10 +1,12 @@
 // The products of a small backward: deltaX = deltaZ W and deltaW = deltaZ^T X where a tile kernel's beginning, end and second
-// launch would be most of the time. Both operands straight from memory, no LDS before the end, one launch.
+// launch would be most of the time. Both operands straight from memory, no LDS before the end, one launch, or a second where a long
+// reduction of few results is cut over workgroups.
 //
-// A workgroup of eight wavefronts computes 32 x 64 of C[m, n] = sum_k A(m, k) B(n, k); every wavefront takes every eighth
+// A workgroup of eight wavefronts computes 32 x 64 or 16 x 32 of C[m, n] = sum_k A(m, k) B(n, k); every wavefront takes every eighth
 // chunk of k for the whole of it, and the eight sums are added through LDS in a fixed order. B has k as its rows: a lane loads
-// four columns n0 + 4 (lane % 16) .. + 3 of a row, which are its elements of four MFMAs (column 4 i + j for i = lane % 16 of
-// MFMA j); A with k as its rows likewise with two columns, else a lane's consecutive k of a row.
+// TN columns n0 + TN (lane % 16) .. of a row, which are its elements of TN MFMAs (column TN i + j for i = lane % 16 of
+// MFMA j); A with k as its rows likewise with TM columns, else a lane's consecutive k of a row. Bound by what a compute unit
+// loads (35 to 40 bytes a nanosecond), in fp32 with the larger tile by the MFMAs.
 //   fp32: chunks of 16 k, v_mfma_f32_16x16x4_f32, the lane's k being 4 (lane / 16) + s in the s-th: plain fp32 products;
 //   bf16: chunks of 32 k, v_mfma_f32_16x16x32_bf16, eight k a lane, brought together from eight rows by byte permutes.
 // Rows beyond K are zeros, rows and columns of C beyond its edge are not stored (their loads stay inside the operand).

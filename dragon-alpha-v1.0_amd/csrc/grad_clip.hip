@@ -8,7 +8,7 @@
 // the norm's bits do not change from run to run.
 // Scaling goes through the pieces from the last to the first, so what the first pass read last is still in the last-level cache
 // (256 MB).
-// Measured: 162 tensors, 102 MB of fp32, squares / norm / scaling 19 / 4 / 39 us (5.4 and 5.2 TB/s);
+// Measured: 162 tensors, 102 MB of fp32, squares / norm / scaling 19 / 4 / 36 us (5.4 and 5.7 TB/s);
 // 48 tensors, 418 MB of bf16, 99 / 5 / 135 us (4.2 and 6.2 TB/s, the writes of the pass before still on their way to memory in the
 // first).
 #include "dense_common.hpp"
