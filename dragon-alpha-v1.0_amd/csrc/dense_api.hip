@@ -48,7 +48,7 @@ struct Scratch {
 bool sizes_served(int type, int64_t N, int64_t IC, int64_t OC, int pair = 1)
 {
     if (type != ALPHA_DENSE_F32 && type != ALPHA_DENSE_BF16) return false;
-    if (N < 0 || IC < 0 || OC < 0 || IC > (1 << 22) || pair * OC > (1 << 22)) return false;   // (a pair's deltaZ lie side by side)
+    if (N < 0 || N >= (1 << 30) || IC < 0 || OC < 0 || IC > (1 << 22) || pair * OC > (1 << 22)) return false;   // (a pair's deltaZ lie side by side)
     // packed tensors of at most 2^34 elements: their 16-byte chunks are counted in 31 bits
     return N * round8(IC) < (1l << 34) && 2 * N * round8(OC) < (1l << 34) && OC * round8(IC) < (1l << 34);
 }
@@ -149,6 +149,7 @@ int quads_aligned(int type, std::initializer_list<const void *> p, std::initiali
 
 // ---- workspaces: the same sequence of blocks for the query (base NULL) and the call --------------------------------
 struct ForwardRoom {
+    DenseForm form;
     void *X, *W[2];
     float *pieces;
     size_t piece_bytes, total;
@@ -157,7 +158,8 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
 {
     Scratch ws(base);
     ForwardRoom r{};
-    if (dense_forward_form(type == ALPHA_DENSE_F32, gated, N, OC, IC) != DENSE_TILES_FORM) return r;   // operands as they are, no pieces
+    r.form = dense_forward_form(type == ALPHA_DENSE_F32, gated, N, OC, IC);
+    if (r.form != DENSE_TILES_FORM) return r;   // operands as they are, no pieces
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
     r.piece_bytes = dense_product_piece_bytes(N, OC, IC, type == ALPHA_DENSE_F32, 1, gated);
@@ -194,10 +196,9 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
 
 // Forward, plain and gated.
 int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, int64_t ldX, const void *W, int64_t ldW, const void *W2, int64_t ldW2,
-            const DenseEpilogue &ep, int N, int IC, int OC, void *workspace)
+            const DenseEpilogue &ep, int N, int IC, int OC, const ForwardRoom &room)
 {
-    const DenseForm form = dense_forward_form(type == ALPHA_DENSE_F32, gated, N, OC, IC);
-    if (form != DENSE_TILES_FORM) {
+    if (room.form != DENSE_TILES_FORM) {
         DenseFewRows a{};
         a.X = X;
         a.ldX = ldX;
@@ -211,9 +212,8 @@ int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, i
         a.N = OC;
         a.K = IC;
         a.ep = ep;
-        return hip_status(form == DENSE_FEW_ROWS ? launch_dense_few_rows(s, a) : launch_dense_short(s, a), fn);
+        return hip_status(room.form == DENSE_FEW_ROWS ? launch_dense_few_rows(s, a) : launch_dense_short(s, a), fn);
     }
-    const ForwardRoom room = forward_room(type, N, IC, OC, gated, workspace);
     DenseProduct p{};
     p.sources = 1;
     p.gated = gated;
@@ -240,9 +240,8 @@ struct BackwardCall {
     int64_t ld_dX, ld_dW[2];
 };
 
-int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardCall &c, int act, float k, int N, int IC, int OC, void *workspace)
+int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardCall &c, int act, float k, int N, int IC, int OC, const BackwardRoom &room)
 {
-    const BackwardRoom room = backward_room(type, N, IC, OC, gated, workspace);
     const bool want_x = c.dX != nullptr && N > 0 && IC > 0, want_w = (c.dW[0] || c.dW[1]) && OC > 0 && IC > 0;
     const bool products = want_x || want_w;
     const int pair = gated ? 2 : 1;
@@ -349,7 +348,9 @@ ALPHA_EXPORT int alpha_matMul_fused(const int64_t *streams, int length, int type
                                     int64_t Y_stride, int N, int IC, int OC, void *workspace, int64_t workspace_bytes)
 {
     const char *fn = __func__;
-    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, alpha_matMul_fused_workspace(type, N, IC, OC)));
+    const bool served = sizes_served(type, N, IC, OC);
+    const ForwardRoom room = served ? forward_room(type, N, IC, OC, 0, workspace) : ForwardRoom{};
+    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, served ? (int64_t)room.total : -1));
     TRY(check_matrix(fn, "X", X, X_stride, N, IC, type, true));
     TRY(check_matrix(fn, "W", W, W_stride, OC, IC, type, true));
     TRY(check_vector(fn, "Bias", Bias, type));
@@ -374,7 +375,7 @@ ALPHA_EXPORT int alpha_matMul_fused(const int64_t *streams, int length, int type
     ep.act = act;
     ep.slope = k;
     ep.vec = quads_aligned(type, {Bias, R, Z, Y}, {R ? R_stride : 0, Z ? Z_stride : 0, Y_stride});
-    return forward(fn, s, type, 0, X, X_stride, W, W_stride, nullptr, 0, ep, N, IC, OC, workspace);
+    return forward(fn, s, type, 0, X, X_stride, W, W_stride, nullptr, 0, ep, N, IC, OC, room);
 }
 
 ALPHA_EXPORT int64_t alpha_dmatMul_fused_workspace(int type, int N, int IC, int OC)
@@ -388,7 +389,9 @@ ALPHA_EXPORT int alpha_dmatMul_fused(const int64_t *streams, int length, int typ
                                      void *workspace, int64_t workspace_bytes)
 {
     const char *fn = __func__;
-    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, alpha_dmatMul_fused_workspace(type, N, IC, OC)));
+    const bool served = sizes_served(type, N, IC, OC);
+    const BackwardRoom room = served ? backward_room(type, N, IC, OC, 0, workspace) : BackwardRoom{};
+    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, served ? (int64_t)room.total : -1));
     TRY(check_matrix(fn, "deltaY", deltaY, deltaY_stride, N, OC, type, true));
     if (act != ALPHA_DENSE_ACT_NONE) TRY(check_matrix(fn, "Z", Z, Z_stride, N, OC, type, true));
     TRY(check_matrix(fn, "X", X, X_stride, N, IC, type, deltaW != nullptr));
@@ -416,7 +419,7 @@ ALPHA_EXPORT int alpha_dmatMul_fused(const int64_t *streams, int length, int typ
     c.dW[0] = deltaW;
     c.ld_dW[0] = deltaW_stride;
     c.dB[0] = deltaB;
-    return backward(fn, s, type, 0, c, act, k, N, IC, OC, workspace);
+    return backward(fn, s, type, 0, c, act, k, N, IC, OC, room);
 }
 
 ALPHA_EXPORT int64_t alpha_gatedMatMul_workspace(int type, int N, int IC, int OC)
@@ -430,7 +433,9 @@ ALPHA_EXPORT int alpha_gatedMatMul(const int64_t *streams, int length, int type,
                                    int64_t workspace_bytes)
 {
     const char *fn = __func__;
-    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, alpha_gatedMatMul_workspace(type, N, IC, OC)));
+    const bool served = sizes_served(type, N, IC, OC, 2);
+    const ForwardRoom room = served ? forward_room(type, N, IC, OC, 1, workspace) : ForwardRoom{};
+    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, served ? (int64_t)room.total : -1));
     TRY(check_matrix(fn, "X", X, X_stride, N, IC, type, true));
     TRY(check_matrix(fn, "Wg", Wg, Wg_stride, OC, IC, type, true));
     TRY(check_matrix(fn, "Wu", Wu, Wu_stride, OC, IC, type, true));
@@ -456,7 +461,7 @@ ALPHA_EXPORT int alpha_gatedMatMul(const int64_t *streams, int length, int type,
     ep.act = act;
     ep.slope = k;
     ep.vec = quads_aligned(type, {Bg, Bu, G, U, H}, {G ? G_stride : 0, U ? U_stride : 0, H_stride});
-    return forward(fn, s, type, 1, X, X_stride, Wg, Wg_stride, Wu, Wu_stride, ep, N, IC, OC, workspace);
+    return forward(fn, s, type, 1, X, X_stride, Wg, Wg_stride, Wu, Wu_stride, ep, N, IC, OC, room);
 }
 
 ALPHA_EXPORT int64_t alpha_dgatedMatMul_workspace(int type, int N, int IC, int OC)
@@ -471,7 +476,9 @@ ALPHA_EXPORT int alpha_dgatedMatMul(const int64_t *streams, int length, int type
                                     int N, int IC, int OC, void *workspace, int64_t workspace_bytes)
 {
     const char *fn = __func__;
-    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, alpha_dgatedMatMul_workspace(type, N, IC, OC)));
+    const bool served = sizes_served(type, N, IC, OC, 2);
+    const BackwardRoom room = served ? backward_room(type, N, IC, OC, 1, workspace) : BackwardRoom{};
+    TRY(check_call(fn, streams, length, type, N, IC, OC, act, k, workspace, workspace_bytes, served ? (int64_t)room.total : -1));
     TRY(check_matrix(fn, "deltaH", deltaH, deltaH_stride, N, OC, type, true));
     TRY(check_matrix(fn, "G", G, G_stride, N, OC, type, true));
     TRY(check_matrix(fn, "U", U, U_stride, N, OC, type, true));
@@ -508,7 +515,7 @@ ALPHA_EXPORT int alpha_dgatedMatMul(const int64_t *streams, int length, int type
     c.ld_dW[1] = deltaWu_stride;
     c.dB[0] = deltaBg;
     c.dB[1] = deltaBu;
-    return backward(fn, s, type, 1, c, act, k, N, IC, OC, workspace);
+    return backward(fn, s, type, 1, c, act, k, N, IC, OC, room);
 }
 
 ALPHA_EXPORT int64_t alpha_gradClip_workspace(int count, const int64_t *lengths)

@@ -149,6 +149,7 @@ struct DenseProduct {
     size_t piece_bytes;
 };
 size_t dense_product_piece_bytes(int M, int N, int K, int f32, int sources, int gated);
+constexpr double DENSE_LEAST_TILES_US = 6.5;                                                         // no estimate of that is less
 double dense_product_us(int M, int N, int K, int f32, int sources, int gated);   // the plan's estimate
 hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p);
 

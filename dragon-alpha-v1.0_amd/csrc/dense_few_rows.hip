@@ -13,6 +13,8 @@
 // Rows may begin at any element and K may be any number.
 #include "dense_direct.hpp"
 
+#include <algorithm>
+
 namespace alpha {
 
 namespace {
@@ -180,6 +182,7 @@ DenseForm dense_forward_form(int f32, int gated, int M, int N, int K)
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
     const double copies = !f32 && K % 8 ? 6.0 + ((double)M + N) * K * 4 / 4e6 : 0.0;
     const double few = dense_few_rows_us(f32, gated, M, N, K), brief = dense_short_us(f32, gated, M, N, K);
+    if (std::min(few, brief) < DENSE_LEAST_TILES_US) return few <= brief ? DENSE_FEW_ROWS : DENSE_SHORT;   // (the plan takes longer than the others)
     const double tiles = dense_product_us(M, N, K, f32, 1, gated) + copies;
     return tiles <= few && tiles <= brief ? DENSE_TILES_FORM : few <= brief ? DENSE_FEW_ROWS : DENSE_SHORT;
 }

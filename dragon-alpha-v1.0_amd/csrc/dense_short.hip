@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void dense_short_kernel(const DenseFewRows a)
 // from about a third of a workgroup per compute unit on what each more of them costs, by its epilogue and by its MFMAs and loads.
 double dense_short_us(int f32, int gated, int M, int N, int K)
 {
-    if (K < (f32 ? 4 : 8) || (M + 63) / 64 > 65535) return 1e30;   // (less than one load; the grid's second dimension)
+    if (K < (f32 ? 4 : 8) || ((long)M + 63) / 64 > 65535) return 1e30;   // (less than one load; the grid's second dimension)
     static constexpr double start[2][2] = {{3.8, 3.15}, {4.2, 3.5}}, piece[2][2] = {{0.95, 0.95}, {1.5, 1.55}};
     static constexpr double group[2][2] = {{1.4, 1.2}, {1.7, 1.3}}, by_k[2][2] = {{0.63, 0.52}, {1.75, 2.1}}, share[2][2] = {{0.3, 0.44}, {0.33, 0.72}};
     const int t = f32 != 0, g = gated != 0, cus = device_cu_count() > 0 ? device_cu_count() : 1;

@@ -222,8 +222,9 @@ bool dense_small_preferred(int f32, int a_t, int M, int N, int K, int sources)
 {
     // (rows of bf16 that are no whole 16-byte chunks are copied for the tile kernels)
     const double copies = !f32 && N % 8 ? 3.0 + (double)K * sources * N * 4 / 4e6 : 0.0;
-    if (N < 4 || K < 1 || (a_t ? M < 2 : K < 8) || (M + 15) / 16 > 65535) return false;   // (65535: the grid's second dimension)
-    return small_plan(f32, M, N, K, sources).us < dense_product_us(M, N, K, f32, sources, 0) + copies;
+    if (N < 4 || K < 1 || (a_t ? M < 2 : K < 8) || ((long)M + 15) / 16 > 65535) return false;   // (65535: the grid's second dimension)
+    const double us = small_plan(f32, M, N, K, sources).us;
+    return us < DENSE_LEAST_TILES_US || us < dense_product_us(M, N, K, f32, sources, 0) + copies;
 }
 
 hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p)

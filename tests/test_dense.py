@@ -127,3 +127,11 @@ def test_a_pair_of_filters_has_half_the_columns():
         for query in (D.gatedMatMul_workspace, D.dgatedMatMul_workspace):
             with pytest.raises(pkg.AlphaConvError):
                 query(code, 8, 8, (1 << 21) + 1)
+
+
+def test_rows_have_a_limit():
+    for query in (D.matMul_fused_workspace, D.dmatMul_fused_workspace, D.gatedMatMul_workspace, D.dgatedMatMul_workspace):
+        for code in (D.F32, D.BF16):
+            assert query(code, (1 << 30) - 1, 4, 2) >= 0
+            with pytest.raises(pkg.AlphaConvError):
+                query(code, 1 << 30, 4, 2)
