@@ -45,7 +45,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_f32_kernel(const D
     constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
     constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT, LOADS = LA + LB;       // 16-byte loads of a thread per step
     constexpr unsigned APLANE = BM * 64, BPLANE = BN * 64, BUFFER = 3 * (APLANE + BPLANE);
-    static_assert(MF == 4 && NF == 4 && NT % 256 == 0, "a wavefront owns 64 x 64");
+    static_assert((MF == 4 || MF == 2) && NF == 4 && NT % 256 == 0, "a wavefront owns 64 or 32 x 64");
+    constexpr int R = MF * NF;     // MFMAs of a product of two parts
     extern __shared__ char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, q = lane >> 4;
@@ -188,41 +189,43 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_f32_kernel(const D
 
     unsigned buffer = 0;
     int kept = 0;          // kleft of the step that `raw` holds
-    auto step = [&](const bf16x8 (&ah)[4], const bf16x8 (&bl)[4], bf16x8 (&next_ah)[4], bf16x8 (&next_bl)[4]) {
+    auto step = [&](const bf16x8 (&ah)[MF], const bf16x8 (&bl)[4], bf16x8 (&next_ah)[MF], bf16x8 (&next_bl)[4]) {
         const unsigned next = BUFFER - buffer;
-        bf16x8 am[4], bm[4], al[4], bh[4];
+        bf16x8 am[MF], bm[4], al[MF], bh[4];
         begin();
-        // runs 1 and 2: 48 MFMAs, 3 LOADS turns of splitting, 16 reads
-        for_each<48>([&](auto index) __attribute__((always_inline)) {
+        // runs 1 and 2: 3 R MFMAs, 3 LOADS turns of splitting, 8 + 2 MF reads
+        for_each<3 * R>([&](auto index) __attribute__((always_inline)) {
             constexpr int x = index;
             for_each<3 * LOADS>([&](auto turn) __attribute__((always_inline)) {
                 constexpr int w = turn;
-                if constexpr (w * 48 / (3 * LOADS) == x) {
+                if constexpr (w * R / LOADS == x) {
                     if constexpr (w % 3 == 0) clear_tail(std::integral_constant<int, w / 3>{}, kept);
                     split(std::integral_constant<int, w / 3>{}, std::integral_constant<int, w % 3>{}, next);
                     if constexpr (w % 3 == 2) load(std::integral_constant<int, w / 3>{});
                 }
             });
-            if constexpr (x < 16) {
-                if constexpr (x % 2 == 0 && x / 2 < 4) bm[x / 2] = read_b(buffer, 1, x / 2);
-                if constexpr (x % 2 == 0 && x / 2 >= 4) am[x / 2 - 4] = read_a(buffer, 1, x / 2 - 4);
+            if constexpr (x < R) {
+                constexpr int every = MF / 2, r = x / every;
+                if constexpr (x % every == 0 && r < 4) bm[r] = read_b(buffer, 1, r);
+                if constexpr (x % every == 0 && r >= 4 && r < 4 + MF) am[r - 4] = read_a(buffer, 1, r - 4);
             } else {
-                if constexpr (x % 2 == 0 && x < 24) bh[(x - 16) / 2] = read_b(buffer, 0, (x - 16) / 2);
-                if constexpr (x % 2 == 0 && x >= 24 && x < 32) al[(x - 24) / 2] = read_a(buffer, 2, (x - 24) / 2);
+                constexpr int r = (x - R) / 2;
+                if constexpr (x % 2 == 0 && r < 4) bh[r] = read_b(buffer, 0, r);
+                if constexpr (x % 2 == 0 && r >= 4 && r < 4 + MF) al[r - 4] = read_a(buffer, 2, r - 4);
             }
-            constexpr int i = x / 4 % 4, j = x % 4;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x < 16 ? bl[j] : bm[j], x < 16 ? ah[i] : x < 32 ? am[i] : ah[i], acc[i][j], 0, 0, 0);
+            constexpr int i = x / 4 % MF, j = x % 4;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x < R ? bl[j] : bm[j], x < R ? ah[i] : x < 2 * R ? am[i] : ah[i], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         });
         kept = kleft;
         lds_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        for_each<48>([&](auto index) __attribute__((always_inline)) {
-            constexpr int x = index;
-            if constexpr (x % 4 == 0 && x < 16) next_bl[x / 4] = read_b(next, 2, x / 4);
-            if constexpr (x % 4 == 0 && x >= 16 && x < 32) next_ah[x / 4 - 4] = read_a(next, 0, x / 4 - 4);
-            constexpr int i = x / 4 % 4, j = x % 4;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bh[j], x < 16 ? al[i] : x < 32 ? am[i] : ah[i], acc[i][j], 0, 0, 0);
+        for_each<3 * R>([&](auto index) __attribute__((always_inline)) {
+            constexpr int x = index, r = x / 4;
+            if constexpr (x % 4 == 0 && r < 4) next_bl[r] = read_b(next, 2, r);
+            if constexpr (x % 4 == 0 && r >= 4 && r < 4 + MF) next_ah[r - 4] = read_a(next, 0, r - 4);
+            constexpr int i = r % MF, j = x % 4;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bh[j], x < R ? al[i] : x < 2 * R ? am[i] : ah[i], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         });
         buffer = next;
@@ -240,12 +243,11 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_f32_kernel(const D
     });
     kept = kleft;
     lds_barrier();
-    bf16x8 ah0[4], bl0[4], ah1[4], bl1[4];
+    bf16x8 ah0[MF], bl0[4], ah1[MF], bl1[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        bl0[i] = read_b(0, 2, i);
-        ah0[i] = read_a(0, 0, i);
-    }
+    for (int i = 0; i < 4; i++) bl0[i] = read_b(0, 2, i);
+#pragma unroll
+    for (int i = 0; i < MF; i++) ah0[i] = read_a(0, 0, i);
     for (int t = 0; t < left; t += 2) {   // (an odd number of steps ends with one of zeros)
         step(ah0, bl0, ah1, bl1);
         step(ah1, bl1, ah0, bl0);

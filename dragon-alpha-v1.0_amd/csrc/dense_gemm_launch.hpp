@@ -32,7 +32,7 @@ inline hipError_t launch_dense_tile_any(hipStream_t s, const DenseTileArgs &a, D
 {
     if (f32) {
         if (tile == DENSE_TILE_256_128) return launch_dense_tile<dense_tile_f32_kernel<AT, BT, GATED, 256, 128, 4, 2>>(s, a, 512, 2 * 3 * (256 + 128) * 64);
-        return launch_dense_tile<dense_tile_f32_kernel<AT, BT, GATED, 128, 128, 2, 2>>(s, a, 256, 2 * 3 * (128 + 128) * 64);
+        return launch_dense_tile<dense_tile_f32_kernel<AT, BT, GATED, 128, 128, 4, 2>>(s, a, 512, 2 * 3 * (128 + 128) * 64);
     }
     switch (tile) {
     case DENSE_TILE_256: return launch_dense_tile<dense_tile_kernel<AT, BT, GATED, 256, 256, 2, 4, 4>>(s, a, 512, 4 * (256 + 256) * 64);
