@@ -69,10 +69,10 @@ size_t piece_bytes(const Plan &p) { return ((size_t)p.tiles_m * p.tiles_n - p.wh
 // all, where there are few) with their reduction cut so that they fill the device once more. The choice is the least of an
 // estimate of the device's time; its constants were measured on products of 256 x 256 x 256 to 8192 x 4096 x 4096: a
 // workgroup's step with the device nearly empty and full, bf16 (256 / 256 x 128 / 128) 0.57 / 0.34 / 0.30 and 0.70 / 0.48 /
-// 0.54 us, the last with two workgroups on a compute unit; fp32 (256 x 128 / 128) 2.05 / 1.5 and 2.55 / 1.75.
+// 0.54 us, the last with two workgroups on a compute unit; fp32 (256 x 128 / 128) 2.05 / 1.3 and 2.55 / 1.5.
 Plan make_plan(int M, int N, int K, int f32, int sources, int gated, size_t room)
 {
-    static constexpr double empty[2][DENSE_TILES] = {{0.57, 0.34, 0.30}, {0, 2.05, 1.5}}, full[2][DENSE_TILES] = {{0.70, 0.48, 0.54}, {0, 2.55, 1.75}};
+    static constexpr double empty[2][DENSE_TILES] = {{0.57, 0.34, 0.30}, {0, 2.05, 1.3}}, full[2][DENSE_TILES] = {{0.70, 0.48, 0.54}, {0, 2.55, 1.5}};
     static constexpr double fixed[DENSE_TILES] = {6.5, 5.0, 3.0};
     const int cus = std::max(1, device_cu_count());
     const int nk = std::max(1, (K + 31) / 32), steps = nk * sources;
