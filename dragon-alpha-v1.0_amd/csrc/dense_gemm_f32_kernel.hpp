@@ -2,18 +2,19 @@
 // the fp32 one. x = h + m + l exactly, three bf16 of 8 significant bits each (rounded to nearest, signs of their own); of the
 // nine products of parts the six above 2^-24 of the whole are summed, small ones first, in fp32:
 //     x y = h l' + m m' + h m' + l h' + m h' + h h'   (left out: m l', l m', l l', together below 2^-23 |x y|).
-// 2.5 PF / 6 = 417 TF bound, 157 TF through v_mfma_f32_16x16x4_f32. Measured: 4096 x 1024 x 4096 with GELU and both outputs 178 us,
-// 193 TF; the matrix pipe is busy 54 % of the cycles at 1.84 GHz, the rest is the splitting, which it waits for.
+// 2.5 PF / 6 = 417 TF bound, 157 TF through v_mfma_f32_16x16x4_f32. Measured: 4096 x 1024 x 4096 with GELU and both outputs 185 us,
+// 185 TF; the matrix pipe is busy 54 % of the cycles at 1.84 GHz, the rest is the splitting, which it waits for.
 //
 // A workgroup takes BM x BN of C in steps of 32 k. An element is split once per workgroup: loaded to registers (128-bit buffer
 // loads, a step ahead), split, and written to LDS as three bf16 planes of the layout that dense_gemm_kernel.hpp describes, in
 // two buffers. Operands are read in place, whatever their stride, alignment and storage. A step has three runs of MFMAs - by
-// l', m' and h' of B, 16 + 32 + 48 per wavefront of 64 x 64 -, and a run's fragments are read during the run before:
+// l', m' and h' of B, 16 + 32 + 48 per wavefront of 64 x 64, half of them of 32 x 64 -, and a run's fragments are read during the run
+// before:
 //     run 1: h l'              reads m', m        splits and writes the next step's elements, asks for those of the step after
 //     run 2: m m', h m'        reads h', l          (the same, on to the barrier)
 //     barrier: every read of this step's planes and every write of the next step's is done
 //     run 3: l h', m h', h h'  reads the next step's l', h
-// so the one barrier of a step (3072 cycles of MFMAs per SIMD) stands between MFMAs whose operands are in registers.
+// so the one barrier of a step (256 x 128: 3072 cycles of MFMAs per SIMD) stands between MFMAs whose operands are in registers.
 // An infinity or NaN makes NaN (h - h), and so does a value that rounds up beyond bf16's range: a NaN result is computed again
 // in plain fp32 (dense_element).
 #pragma once
