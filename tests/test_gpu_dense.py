@@ -748,3 +748,65 @@ def test_backward_of_few_rows(kind, n, ic, oc):
 def test_backward_of_long_sums_of_few_results(kind, n, ic, oc, pad):
     check_backward(kind, n, ic, oc, D.ACT_SIGMOID, pad=pad)
     check_gated_backward(kind, n, ic, oc, pad=pad)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,ic,oc", [(64, 320, 3136), (4416, 33, 35), (2, 5, 4099), (200, 64, 4400), (1100, 96, 1030), (129, 2049, 513), (2000, 1500, 700)])
+def test_nothing_is_written_behind_a_workspace_of_any_form(kind, n, ic, oc):
+    code, dtype = TYPES[kind]
+    x, w, u = matrix(n, ic, dtype, 1), matrix(oc, ic, dtype, 2), matrix(oc, ic, dtype, 3)
+    dy, z = matrix(n, oc, dtype, 4), matrix(n, oc, dtype, 5)
+    dx, dw, du, db = Out(n, ic, dtype), Out(oc, ic, dtype), Out(oc, ic, dtype), Out(1, oc, dtype)
+    y = Out(n, oc, dtype)
+    p = lambda t: t.data_ptr()
+    calls = [
+        (D.matMul_fused_workspace, lambda ws: D.matMul_fused(stream(), 1, code, p(x), ic, p(w), ic, 0, D.ACT_SILU, 0.0, 0, 0, 0, 0, y.ptr(), oc, n, ic, oc, *ws), (y,)),
+        (D.gatedMatMul_workspace, lambda ws: D.gatedMatMul(stream(), 1, code, p(x), ic, p(w), ic, 0, p(u), ic, 0, D.ACT_SILU, 0.0, 0, 0, 0, 0, y.ptr(), oc, n, ic, oc, *ws), (y,)),
+        (D.dmatMul_fused_workspace, lambda ws: D.dmatMul_fused(stream(), 1, code, p(dy), oc, p(z), oc, D.ACT_SILU, 0.0, p(x), ic, p(w), ic, dx.ptr(), ic, dw.ptr(), ic,
+                                                               db.ptr(), n, ic, oc, *ws), (dx, dw, db)),
+        (D.dgatedMatMul_workspace, lambda ws: D.dgatedMatMul(stream(), 1, code, p(dy), oc, p(z), oc, p(dy), oc, D.ACT_SILU, 0.0, p(x), ic, p(w), ic, p(u), ic, dx.ptr(), ic,
+                                                             dw.ptr(), ic, du.ptr(), ic, db.ptr(), 0, n, ic, oc, *ws), (dx, dw, du, db)),
+    ]
+    for query, call, outputs in calls:
+        need = query(code, n, ic, oc)
+        got = []
+        for poison in (0xA5, 0x5A):     # whatever lay there before
+            ws = torch.full((need + 65536,), poison, dtype=torch.uint8, device="cuda")
+            call((ws.data_ptr(), need))
+            got.append([o.get() for o in outputs])
+            assert bool((ws[need:] == poison).all()), query
+        for a, b in zip(*got):
+            assert bool((a == b).all()) and not bool(a.isnan().any()), query
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,ic,oc", [(64, 320, 3136), (384, 96, 1100), (20, 2001, 300), (5, 1217, 895)])
+def test_calls_replayed_from_a_graph_between_eager_ones(kind, n, ic, oc):
+    code, dtype = TYPES[kind]
+    x, w, dy = matrix(n, ic, dtype, 1), matrix(oc, ic, dtype, 2, ic ** -0.5), matrix(n, oc, dtype, 3)
+    b = matrix(1, oc, dtype, 4)[0]
+    z, y = torch.empty(n, oc, dtype=dtype, device="cuda"), torch.empty(n, oc, dtype=dtype, device="cuda")
+    dx, dw, db = torch.empty(n, ic, dtype=dtype, device="cuda"), torch.empty(oc, ic, dtype=dtype, device="cuda"), torch.empty(oc, dtype=dtype, device="cuda")
+    wf, nf = workspace(D.matMul_fused_workspace, code, n, ic, oc)
+    wb, nb = workspace(D.dmatMul_fused_workspace, code, n, ic, oc)
+
+    def step():
+        D.matMul_fused(stream(), 1, code, x.data_ptr(), ic, w.data_ptr(), ic, b.data_ptr(), D.ACT_GELU, 0.0, 0, 0, z.data_ptr(), oc, y.data_ptr(), oc, n, ic, oc, wf.data_ptr(), nf)
+        D.dmatMul_fused(stream(), 1, code, dy.data_ptr(), oc, z.data_ptr(), oc, D.ACT_GELU, 0.0, x.data_ptr(), ic, w.data_ptr(), ic, dx.data_ptr(), ic, dw.data_ptr(), ic,
+                        db.data_ptr(), n, ic, oc, wb.data_ptr(), nb)
+
+    outputs = (z, y, dx, dw, db)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for turn in range(3):
+        x.copy_(matrix(n, ic, dtype, 10 + turn))
+        step()
+        torch.cuda.synchronize()
+        want = [t.clone() for t in outputs]
+        for t in outputs:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(bool((t == e).all()) for t, e in zip(outputs, want)), turn
