@@ -6,7 +6,8 @@ import ctypes
 from . import native
 
 _I, _L, _P, _F = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
-_bound = False
+_functions = {}          # bound entries by name, once the library is loaded
+_ONE = _L * 1
 
 # S = stream array, i = int, l = int64, f = float, p = device pointer; n, q, t = host arrays of int, int64, addresses
 _SIGS = {
@@ -25,21 +26,19 @@ def exported_symbols():
     return sorted(list(_SIGS) + list(_SIZES) + ["alpha_gradClip_workspace", "alpha_dense_last_error"])
 
 
-def _lib():
-    global _bound
+def _bind():
     L = native.lib()
-    if not _bound:
-        for name, sig in _SIGS.items():
-            getattr(L, name).argtypes = [_CT[c] for c in sig]
-            getattr(L, name).restype = _I
-        for name in _SIZES:
-            getattr(L, name).argtypes = [_I] * 4
-            getattr(L, name).restype = _L
-        L.alpha_gradClip_workspace.argtypes = [_I, ctypes.POINTER(_L)]
-        L.alpha_gradClip_workspace.restype = _L
-        L.alpha_dense_last_error.restype = ctypes.c_char_p
-        _bound = True
-    return L
+    for name, sig in _SIGS.items():
+        getattr(L, name).argtypes = [_CT[c] for c in sig]
+        getattr(L, name).restype = _I
+    for name in _SIZES:
+        getattr(L, name).argtypes = [_I] * 4
+        getattr(L, name).restype = _L
+    L.alpha_gradClip_workspace.argtypes = [_I, ctypes.POINTER(_L)]
+    L.alpha_gradClip_workspace.restype = _L
+    L.alpha_dense_last_error.restype = ctypes.c_char_p
+    _functions.update({name: getattr(L, name) for name in exported_symbols()})
+    return _functions
 
 
 def _array(kind, values):
@@ -48,13 +47,13 @@ def _array(kind, values):
 
 def _call(name, streams, *args):
     """`args` as ctypes takes them for the signature: integers, floats, arrays."""
-    rc = getattr(_lib(), name)((_L * max(1, len(streams)))(*streams), *args)
+    rc = (_functions or _bind())[name](_ONE(streams[0]) if len(streams) == 1 else (_L * max(1, len(streams)))(*streams), *args)
     if rc != 0:
-        raise native.AlphaConvError("%s failed (%d): %s" % (name, rc, native.lib().alpha_dense_last_error().decode()))
+        raise native.AlphaConvError("%s failed (%d): %s" % (name, rc, _functions["alpha_dense_last_error"]().decode()))
 
 
 def _workspace(name, *args):
-    n = getattr(_lib(), name)(*args)
+    n = (_functions or _bind())[name](*args)
     if n < 0:
         raise native.AlphaConvError("%s: size out of range %s" % (name, args))
     return n
