@@ -183,12 +183,18 @@ BackwardRoom backward_room(int type, int N, int IC, int OC, int gated, void *bas
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < pair; i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
     r.sums = ws.take<float>(dense_delta_sum_bytes(N, OC, gated));
+    // two small products are one launch, so their pieces are there at a time
+    struct Pieces {
+        size_t small, tiles;
+    };
     auto pieces = [&](int a_t, int M, int N, int K, int sources) {
         const int f32 = type == ALPHA_DENSE_F32;
-        return dense_small_preferred(f32, a_t, M, N, K, sources) ? dense_small_piece_bytes(f32, M, N, K, sources) : dense_product_piece_bytes(M, N, K, f32, sources, 0);
+        if (dense_small_preferred(f32, a_t, M, N, K, sources)) return Pieces{dense_small_piece_bytes(f32, M, N, K, sources), 0};
+        return Pieces{0, dense_product_piece_bytes(M, N, K, f32, sources, 0)};
     };
     // a gated pair's filter gradients are one stacked product, or one of them alone
-    r.piece_bytes = std::max({pieces(0, N, IC, OC, pair), pieces(1, OC, IC, N, 1), gated ? pieces(1, (int)round8(OC) + OC, IC, N, 1) : (size_t)0});
+    const Pieces x = pieces(0, N, IC, OC, pair), w = pieces(1, OC, IC, N, 1), both = gated ? pieces(1, (int)round8(OC) + OC, IC, N, 1) : Pieces{0, 0};
+    r.piece_bytes = std::max({x.small + std::max(w.small, both.small), x.tiles, w.tiles, both.tiles});
     r.pieces = ws.take<float>(r.piece_bytes);
     r.total = ws.at;
     return r;
@@ -282,6 +288,7 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
     p.f32 = d.f32;
     p.pieces = room.pieces;
     p.piece_bytes = room.piece_bytes;
+    DenseProduct small_x{};      // waits for deltaW
     if (want_x) {   // deltaX[n, ic] = sum over oc (and over both filters)
         p.A = delta;
         p.sources = pair;
@@ -299,8 +306,11 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
             const bool pack = strides || (!small && (!in_place(type, c.W[0], c.ldW[0], IC) || (gated && !in_place(type, c.W[1], c.ldW[1], IC))));
             for (int i = 0; i < pair; i++) TRY(operand(fn, s, type, c.W[i], c.ldW[i], OC, IC, room.W[i], pack, p.B, i));
         }
-        TRY(hip_status(small ? launch_dense_small(s, p) : launch_dense_product(s, p), fn));
+        if (!small) TRY(hip_status(launch_dense_product(s, p), fn));
+        else if (want_w) small_x = p;
+        else TRY(hip_status(launch_dense_small(s, &p, nullptr), fn));
     }
+    const DenseProduct *waiting = small_x.M > 0 ? &small_x : nullptr;
     if (want_w) {   // deltaW[oc, ic] = sum over n; both filters' as one product over the pair's columns
         p.A = delta;
         p.B = DenseOperand{};
@@ -325,7 +335,12 @@ int backward(const char *fn, hipStream_t s, int type, int gated, const BackwardC
         }
         const bool small = dense_small_preferred(p.f32, 1, p.M, p.N, p.K, 1);
         if (N > 0) TRY(operand(fn, s, type, c.X, c.ldX, N, IC, room.X, !small && !in_place(type, c.X, c.ldX, IC), p.B, 0));
-        TRY(hip_status(small ? launch_dense_small(s, p) : launch_dense_product(s, p), fn));
+        if (small) {
+            TRY(hip_status(launch_dense_small(s, waiting, &p), fn));
+        } else {
+            if (waiting) TRY(hip_status(launch_dense_small(s, waiting, nullptr), fn));
+            TRY(hip_status(launch_dense_product(s, p), fn));
+        }
     }
     return 0;
 }

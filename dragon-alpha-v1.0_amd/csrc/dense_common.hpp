@@ -173,7 +173,7 @@ hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);
 // Small products of a backward (B with k as its rows), operands as they are, no pieces (dense_small.hip).
 size_t dense_small_piece_bytes(int f32, int M, int N, int K, int sources);
 bool dense_small_preferred(int f32, int a_t, int M, int N, int K, int sources);
-hipError_t launch_dense_small(hipStream_t s, const DenseProduct &p);
+hipError_t launch_dense_small(hipStream_t s, const DenseProduct *px, const DenseProduct *pw);   // deltaX and deltaW, one may be null
 
 // dst <- src[rows, cols]; row stride ld (multiple of 8), columns cols .. ld zero.
 hipError_t launch_dense_pack(hipStream_t s, int f32, const void *src, long src_ld, long rows, int cols, void *dst, long ld);
