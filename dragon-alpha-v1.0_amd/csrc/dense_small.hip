@@ -29,6 +29,7 @@ struct DenseSmallArgs {
     int per;              // chunks of a workgroup
     int cuts;             // pieces of the reduction
     int across, down;     // workgroups of a piece
+    FastDiv by_row, by_piece;
     float *pieces;        // cuts > 1: [cuts][M][columns, a multiple of 4]
     DenseEpilogue ep;
 };
@@ -42,8 +43,8 @@ static __device__ __forceinline__ void small_tile(const DenseSmallArgs &a, int b
     constexpr int CHUNK = sizeof(T) == 4 ? 16 : 32, V = CHUNK / 4;   // k of a chunk, of a lane
     floatx4(*const part)[TM * TN][64] = reinterpret_cast<floatx4(*)[TM * TN][64]>(lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
-    const int piece = block / (a.across * a.down), at_tile = block % (a.across * a.down);
-    const int m0 = at_tile / a.across * SMALL_M, n0 = at_tile % a.across * SMALL_N;
+    const int piece = a.cuts > 1 ? (int)fdiv((uint32_t)block, a.by_piece) : 0, tile = block - piece * (int)a.by_piece.d;
+    const int row = (int)fdiv((uint32_t)tile, a.by_row), m0 = row * SMALL_M, n0 = (tile - row * (int)a.by_row.d) * SMALL_N;
     floatx4 acc[TM][TN];
 #pragma unroll
     for (int t = 0; t < TM; t++)
@@ -131,10 +132,10 @@ static __device__ __forceinline__ void small_tile(const DenseSmallArgs &a, int b
     __syncthreads();
     // MFMA (t, j): lane (l16, q), element e: column i = 4 q + e of the MFMA, which is n0 + TN i + j; row l16, which is m0 + 16 t +
     // l16, or m0 + TM l16 + t where A has k as its rows. A thread takes TN consecutive columns of a row: one i, j = 0 .. TN - 1.
-    const int row = threadIdx.x >> 4, i = threadIdx.x & 15;
-    const int m = m0 + row, n = n0 + TN * i;
-    if (row >= SMALL_M || m >= a.M || n >= a.N) return;
-    const int t = AT ? row % TM : row >> 4, at = (i >> 2) * 16 + (AT ? row / TM : row & 15);
+    const int part_row = threadIdx.x >> 4, i = threadIdx.x & 15;
+    const int m = m0 + part_row, n = n0 + TN * i;
+    if (part_row >= SMALL_M || m >= a.M || n >= a.N) return;
+    const int t = AT ? part_row % TM : part_row >> 4, at = (i >> 2) * 16 + (AT ? part_row / TM : part_row & 15);
     float v[TN];
 #pragma unroll
     for (int j = 0; j < TN; j++) {
@@ -273,6 +274,8 @@ DenseSmallArgs small_args(const DenseProduct &p, float *&pieces, bool &big)
     big = !plan.few;
     a.across = (p.N + (big ? 63 : 31)) / (big ? 64 : 32);
     a.down = (p.M + (big ? 31 : 15)) / (big ? 32 : 16);
+    a.by_row = make_fastdiv((uint32_t)a.across);
+    a.by_piece = make_fastdiv((uint32_t)std::min<long>((long)a.across * a.down, (1l << 31) - 1));
     a.pieces = pieces;
     if (plan.pieces > 1) pieces += (long)plan.pieces * p.M * ((p.N + 3) & ~3);
     return a;
