@@ -14,7 +14,7 @@
 //     run 2: m m', h m'        reads h', l          (the same, on to the barrier)
 //     barrier: every read of this step's planes and every write of the next step's is done
 //     run 3: l h', m h', h h'  reads the next step's l', h
-// so the one barrier of a step (256 x 128: 3072 cycles of MFMAs per SIMD) stands between MFMAs whose operands are in registers.
+// so the one barrier of a step (256 x 128: 192 MFMAs per SIMD) stands between MFMAs whose operands are in registers.
 // An infinity or NaN makes NaN (h - h), and so does a value that rounds up beyond bf16's range: a NaN result is computed again
 // in plain fp32 (dense_element).
 #pragma once
