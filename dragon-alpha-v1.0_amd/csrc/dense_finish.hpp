@@ -68,9 +68,10 @@ static __device__ __forceinline__ void edge_store(T *p, int left, const float (&
 }
 
 // The epilogues of R consecutive columns n .. n+R-1 of row m. WHOLE: all of them exist and groups of four are aligned; else the
-// `left` first. FULL: all of the epilogue; else only the store (the products of a backward).
+// `left` first. FULL: all of the epilogue; else only the store (the products of a backward). `ahead`: the residual's elements, where they
+// have been loaded before.
 template <typename T, int R, bool FULL, bool WHOLE>
-static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n, int left = R)
+static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, float (&v)[R], long m, int n, int left = R, const T *ahead = nullptr)
 {
     const bool second = !FULL && ep.row2 > 0 && m >= ep.row2;
     if (!FULL && ep.row2 > 0 && !second && m >= ep.rows1) return;   // a row between two stacked products
@@ -87,7 +88,14 @@ static __device__ __forceinline__ void dense_finish(const DenseEpilogue &ep, flo
         const T *bias = static_cast<const T *>(ep.bias), *res = static_cast<const T *>(ep.R);
         T *Z = static_cast<T *>(ep.Z);
         float t[R], r[R];
-        if (res) load(res + m * ep.ldR + n, r);
+        if (res) {
+            if (ahead) {
+#pragma unroll
+                for (int e = 0; e < R; e++) r[e] = (float)ahead[e];
+            } else {
+                load(res + m * ep.ldR + n, r);
+            }
+        }
         if (bias) {
             load(bias + n, t);
 #pragma unroll

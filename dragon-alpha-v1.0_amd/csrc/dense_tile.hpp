@@ -91,6 +91,7 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
 {
     constexpr int TM = BM / WM, TN = BN / WN, MF = TM / 16;
     constexpr bool FULL = !BT;     // B with k as its rows: a backward's product
+    constexpr bool AHEAD = FULL && !GATED && BM * BN >= 256 * 256;
     const int l16 = lane & 15, q = lane >> 4;
     constexpr int ROW = 68;                              // floats from row to row: 16 bytes past a multiple of the banks
     constexpr int LANES = GATED ? 4 : 8;                 // lanes of a row, eight columns each (gated: eight of each filter)
@@ -114,20 +115,32 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
             }
         });
         wave_fence();
-#pragma unroll 1
-        for (int y = 0; y < 32; y += AT_ONCE) {
+        // One turn: AT_ONCE rows. AHEAD: a large tile's residual is loaded for all turns first, or each
+        // would wait for its own (8192 x 1024 x 4096 of bf16 with a residual 104 -> 96 us).
+        T ahead[AHEAD ? TURNS : 1][8];
+        const bool use = AHEAD && vec && a.ep.R != nullptr && n + 8 <= a.N && !cut;
+        if constexpr (AHEAD) {
+            if (use) {
+                for_each<TURNS>([&](auto t) __attribute__((always_inline)) {
+                    long m = m0 + wm * TM + i * 16 + t * AT_ONCE + lane / LANES;
+                    if (m >= a.M) m = a.M - 1;
+                    __builtin_memcpy(ahead[t], static_cast<const T *>(a.ep.R) + m * a.ep.ldR + n, 8 * sizeof(T));
+                });
+            }
+        }
+        auto turn = [&](int y, const T *residual) __attribute__((always_inline)) {
             const int row = y + lane / LANES;
             const long m = m0 + wm * TM + i * 16 + row;
             const float *src = part + row * ROW + at;
             float v[8], u[8];
             run_load(src, v);
             if constexpr (GATED) run_load(src + 32, u);
-            if (m >= a.M || n >= a.N) continue;
+            if (m >= a.M || n >= a.N) return;
             if (cut) {
                 float *dst = a.pieces + (((long)piece * cut_tiles + cut_tile) * BM + (wm * TM + i * 16 + row)) * BN + wn * TN + at;
                 run_store(dst, v);
                 if constexpr (GATED) run_store(dst + 32, u);
-                continue;
+                return;
             }
             if constexpr (__is_same(T, float)) {
                 float sum = 0.f;
@@ -135,17 +148,23 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
                 for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
                 if (sum != sum) {   // (also where infinities of both signs meet: no harm)
                     again |= 1u << (i / 2 * TURNS + y / AT_ONCE);
-                    continue;
+                    return;
                 }
             }
             if (vec && n + 8 <= a.N) {
                 if constexpr (GATED) dense_finish_gated<T, 8, true>(a.ep, v, u, m, n);
-                else dense_finish<T, 8, FULL, true>(a.ep, v, m, n);
+                else dense_finish<T, 8, FULL, true>(a.ep, v, m, n, 8, residual);
             } else {
                 const int left = a.N - n < 8 ? a.N - n : 8;
                 if constexpr (GATED) dense_finish_gated<T, 8, false>(a.ep, v, u, m, n, left);
                 else dense_finish<T, 8, FULL, false>(a.ep, v, m, n, left);
             }
+        };
+        if (use) {
+            for_each<AHEAD ? TURNS : 0>([&](auto t) __attribute__((always_inline)) { turn(t * AT_ONCE, ahead[t]); });
+        } else {
+#pragma unroll 1
+            for (int y = 0; y < 32; y += AT_ONCE) turn(y, nullptr);
         }
         wave_fence();
     }

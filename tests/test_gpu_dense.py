@@ -810,3 +810,10 @@ def test_calls_replayed_from_a_graph_between_eager_ones(kind, n, ic, oc):
         graph.replay()
         torch.cuda.synchronize()
         assert all(bool((t == e).all()) for t, e in zip(outputs, want)), turn
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("size", [(4096, 512, 4096), (4100, 256, 4104), (8000, 96, 2052)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_residual_of_large_tiles(kind, size, in_place):
+    check_forward(kind, *size, act=D.ACT_SILU, residual=True, in_place=in_place)
