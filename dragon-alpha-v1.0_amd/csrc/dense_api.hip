@@ -159,7 +159,12 @@ ForwardRoom forward_room(int type, int N, int IC, int OC, int gated, void *base)
     Scratch ws(base);
     ForwardRoom r{};
     r.form = dense_forward_form(type == ALPHA_DENSE_F32, gated, N, OC, IC);
-    if (r.form != DENSE_TILES_FORM) return r;   // operands as they are, no pieces
+    if (r.form != DENSE_TILES_FORM) {   // operands as they are
+        if (r.form == DENSE_FEW_ROWS) r.piece_bytes = dense_few_rows_piece_bytes(type == ALPHA_DENSE_F32, gated, N, OC, IC);
+        r.pieces = ws.take<float>(r.piece_bytes);
+        r.total = ws.at;
+        return r;
+    }
     r.X = ws.take<void>(packed_bytes(type, N, IC));
     for (int i = 0; i < (gated ? 2 : 1); i++) r.W[i] = ws.take<void>(packed_bytes(type, OC, IC, gated));
     r.piece_bytes = dense_product_piece_bytes(N, OC, IC, type == ALPHA_DENSE_F32, 1, gated);
@@ -218,6 +223,8 @@ int forward(const char *fn, hipStream_t s, int type, int gated, const void *X, i
         a.N = OC;
         a.K = IC;
         a.ep = ep;
+        a.pieces = room.pieces;
+        a.piece_bytes = room.piece_bytes;
         return hip_status(room.form == DENSE_FEW_ROWS ? launch_dense_few_rows(s, a) : launch_dense_short(s, a), fn);
     }
     DenseProduct p{};

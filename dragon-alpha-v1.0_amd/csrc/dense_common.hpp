@@ -160,12 +160,16 @@ struct DenseFewRows {
     int f32, gated;
     int M, N, K;
     DenseEpilogue ep;
+    float *pieces;        // room for the pieces of a cut reduction, `piece_bytes`
+    size_t piece_bytes;
+    int cuts, per;        // set by the launcher
 };
 
 // How a forward product is computed: by tiles, or straight from memory as few rows or as a short reduction.
 enum DenseForm { DENSE_TILES_FORM, DENSE_FEW_ROWS, DENSE_SHORT };
 DenseForm dense_forward_form(int f32, int gated, int M, int N, int K);
 double dense_few_rows_us(int f32, int gated, int M, int N, int K);   // estimates
+size_t dense_few_rows_piece_bytes(int f32, int gated, int M, int N, int K);
 double dense_short_us(int f32, int gated, int M, int N, int K);
 hipError_t launch_dense_short(hipStream_t s, const DenseFewRows &a);
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);

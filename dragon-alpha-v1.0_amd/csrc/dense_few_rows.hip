@@ -1,5 +1,5 @@
-// The dense product for few rows of X or little work: no copy of an operand, one launch, as many bytes in flight as the
-// device takes. A single row reads W once and is bound by that: 1 x 4096 x 4096 bf16 8.1 us, 4.2 TB/s; a gated pair 1 x 2048 x 8192
+// The dense product for few rows of X or little work: no copy of an operand, one launch (two where a long reduction of few workgroups
+// is cut), as many bytes in flight as the device takes. A single row reads W once and is bound by that: 1 x 4096 x 4096 bf16 8.1 us, 4.2 TB/s; a gated pair 1 x 2048 x 8192
 // 12.4 us, 5.4 TB/s. More rows are bound by what a compute unit loads (35 to 40 bytes a nanosecond, whatever is in flight).
 //
 // A workgroup of eight wavefronts computes 16 columns of the output (16 rows of W) for 16, 32 or 64 rows of X; its wavefronts
@@ -54,8 +54,9 @@ __global__ __launch_bounds__(FEW_WAVES * 64, !ODD && !GATED && MB == 4 ? 4 : 2) 
     // (bf16, rows that begin with a word: the last load of a row ends with the word of its last element)
     const int end = sizeof(T) == 2 && !ODD ? (a.K + 1) & ~1 : a.K, last = end - V;
     const int turns = a.K < V ? 0 : (a.K + FEW_WAVES * SPAN - 1) / (FEW_WAVES * SPAN);
-    int turn = turns > 0 ? (int)(blockIdx.x % turns) : 0;
-    for (int t = 0; t < turns; t++) {
+    const int from = blockIdx.z * a.per, to = from + a.per < turns ? from + a.per : turns, count = to - from;
+    int turn = count > 0 ? from + (int)(blockIdx.x % count) : 0;
+    for (int t = 0; t < count; t++) {
         const int k0 = (turn * FEW_WAVES + wave) * SPAN, k = k0 + l16 / C * PIECE;
         if (k0 < a.K) {
             vec vw[G][4], vx[MB][4];
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, !ODD && !GATED && MB == 4 ? 4 : 2) 
                     for (int b = 0; b < MB; b++) acc[g][b] = few_multiply(vw[g][c], vx[b][c], acc[g][b]);
             }
         }
-        turn = turn + 1 == turns ? 0 : turn + 1;
+        turn = turn + 1 == to ? from : turn + 1;
     }
 
     if (a.K < V && wave == 0) {   // less than one load: element by element, zeros behind and in the other lanes' pieces
@@ -123,8 +124,49 @@ __global__ __launch_bounds__(FEW_WAVES * 64, !ODD && !GATED && MB == 4 ? 4 : 2) 
                 v[0] += reinterpret_cast<const float *>(&part[s][b][at])[col & 3];
                 if constexpr (GATED) u[0] += reinterpret_cast<const float *>(&part[s][(GATED ? MB : 0) + b][at])[col & 3];
             }
+        if (a.cuts > 1) {
+            const long columns = (a.N + 3) & ~3;
+            float *to = a.pieces + ((long)blockIdx.z * G * a.M + m) * columns + n0 + col;
+            to[0] = v[0];
+            if constexpr (GATED) to[a.M * columns] = u[0];
+            continue;
+        }
         if constexpr (GATED) dense_finish_gated<T, 1, false>(a.ep, v, u, m, n0 + col);
         else dense_finish<T, 1, true, false>(a.ep, v, m, n0 + col);
+    }
+}
+
+// Adds the pieces of a cut reduction in their order: four columns a thread.
+template <typename T, bool GATED>
+__global__ __launch_bounds__(256) void dense_few_sum_kernel(const DenseFewRows a, FastDiv by_row)
+{
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long m = fdiv((uint32_t)i, by_row), columns = (a.N + 3) & ~3;
+    if (m >= a.M) return;
+    const int n = (int)(i - m * by_row.d) * 4;
+    constexpr int G = GATED ? 2 : 1;
+    float v[G][4];
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[g][e] = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < a.cuts; p++) {
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            // (columns behind the last are not written, and not used)
+            const floatx4 t = quad_load(a.pieces + (((long)p * G + g) * a.M + m) * columns + n);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[g][e] += t[e];
+        }
+    }
+    const int left = a.N - n < 4 ? a.N - n : 4;
+    if constexpr (GATED) {
+        if (a.ep.vec && left == 4) dense_finish_gated<T, 4, true>(a.ep, v[0], v[1], m, n);
+        else dense_finish_gated<T, 4, false>(a.ep, v[0], v[1], m, n, left);
+    } else {
+        if (a.ep.vec && left == 4) dense_finish<T, 4, true, true>(a.ep, v[0], m, n);
+        else dense_finish<T, 4, true, false>(a.ep, v[0], m, n, left);
     }
 }
 
@@ -133,12 +175,11 @@ namespace {
 // Four columns a workgroup or 16, for at most four rows: 16 where the columns make a workgroup per compute unit anyway and four
 // would leave wavefronts without a piece of the reduction, if it is one turn, or a pair of filters to read (bf16, us, 4 / 16
 // columns: 1024 -> 4096 3.8 / 3.3, pair 2048 -> 8192 16.0 / 12.6; 2048 -> 8192 7.8 / 8.5, 4096 -> 4096 7.6 / 8.6, 8192 -> 512 4.7 / 10.6).
-template <typename T>
-bool few_columns(const DenseFewRows &a)
+bool few_columns(int f32, int gated, int M, int N, int K)
 {
-    constexpr int TURN = FEW_WAVES * 4 * 64 / sizeof(T);     // of 16 columns; of four, four times as long
-    const bool filled = (a.N + 15) / 16 >= device_cu_count(), idle = a.K < 4 * TURN;
-    return !(filled && idle && (a.gated || a.K <= TURN));
+    const int turn = FEW_WAVES * 4 * 64 / (f32 ? 4 : 2);     // of 16 columns; of four, four times as long
+    const bool filled = (N + 15) / 16 >= device_cu_count(), idle = K < 4 * turn;
+    return M <= 4 && !(filled && idle && (gated || K <= turn));
 }
 
 }  // namespace
@@ -148,8 +189,11 @@ bool few_columns(const DenseFewRows &a)
 // 1024 k in bf16, 512 k in fp32; what does not fit on the compute units at once takes that times `more` again (two workgroups of
 // at most 128 registers share one). Fewer blocks read W more often and use more compute units: 64 rows of 2000 x 296 take
 // 7.6 / 10.5 / 17.6 us in fp32 with 1 / 2 / 4 blocks, 5.0 / 6.4 / 9.4 in bf16.
+// A long reduction of few workgroups is cut over workgroups, at the cost of a second launch: 8 x 8192 x 1000 fp32 25.4 -> 11.5
+// us. (Only with one block of rows: with more the estimate was 1.5 times too low at 8192 k.)
 struct FewBlocks {
     int blocks;      // of 16 rows a workgroup: 1, 2 or 4
+    int cuts, per;   // pieces of the reduction; turns of a piece
     double us;
 };
 static FewBlocks few_blocks(int f32, int gated, int M, int N, int K)
@@ -159,17 +203,29 @@ static FewBlocks few_blocks(int f32, int gated, int M, int N, int K)
     static constexpr double more[2][2][3] = {{{0.7, 0.75, 0.9}, {0.85, 0.9, 1.45}}, {{0.8, 0.9, 0.9}, {0.95, 0.95, 1.2}}};
     const int t = f32 != 0, g = gated != 0;
     const long cus = device_cu_count() > 0 ? device_cu_count() : 1;
-    const double turns = (double)K / (f32 ? 512 : 1024);
+    const int length = f32 ? 512 : 1024, whole = (K + length - 1) / length;
     const double odd = !f32 && K % 2 ? 1.6 : 1.0;      // (rows one behind the other then begin in the middle of a word)
-    FewBlocks best{4, 1e30};
-    for (int b = 2; b >= 0; b--) {
+    FewBlocks best{4, 1, std::max(1, whole), 1e30};
+    for (int b = M <= 16 ? 0 : 2; b >= 0; b--) {
         const long rows = (M + (16l << b) - 1) / (16l << b), groups = ((long)N + 15) / 16 * rows;
         if (rows > 65535) continue;   // (the grid's second dimension)
-        const double group = group_us[t][g][b] + (turns < 0.25 ? 0.25 : turns) * turn_us[t][g][b];
-        const double us = 2.0 + group * odd * (1.0 + more[t][g][b] * (double)((groups + cus - 1) / cus - 1));
-        if (us < best.us) best = FewBlocks{1 << b, us};
+        for (int cuts = 1; cuts <= (b == 0 ? 8 : 1); cuts *= 2) {
+            const int per = std::max(1, (whole + cuts - 1) / cuts);
+            if (cuts > 1 && (groups * cuts > cus || (whole + per - 1) / per != cuts)) break;
+            const double turns = cuts == 1 ? (double)K / length : per;
+            const double group = group_us[t][g][b] + (turns < 0.25 ? 0.25 : turns) * turn_us[t][g][b];
+            double us = 2.0 + group * odd * (1.0 + more[t][g][b] * (double)((groups * cuts + cus - 1) / cus - 1));
+            if (cuts > 1) us += 2.5 + (double)cuts * M * N * (g ? 16 : 8) / 4.2e6;
+            if (us < best.us) best = FewBlocks{1 << b, cuts, per, us};
+        }
     }
     return best;
+}
+size_t dense_few_rows_piece_bytes(int f32, int gated, int M, int N, int K)
+{
+    if (few_columns(f32, gated, M, N, K)) return 0;
+    const FewBlocks plan = few_blocks(f32, gated, M, N, K);
+    return plan.cuts > 1 ? (size_t)plan.cuts * (gated ? 2 : 1) * M * ((N + 3) & ~3) * 4 : 0;
 }
 double dense_few_rows_us(int f32, int gated, int M, int N, int K) { return few_blocks(f32, gated, M, N, K).us; }
 
@@ -190,19 +246,32 @@ DenseForm dense_forward_form(int f32, int gated, int M, int N, int K)
 namespace {
 
 template <typename T, bool ODD, bool GATED>
-hipError_t launch_few(hipStream_t s, const DenseFewRows &a)
+hipError_t launch_few(hipStream_t s, const DenseFewRows &given)
 {
-    const dim3 block(FEW_WAVES * 64);
+    DenseFewRows a = given;
+    const bool f32 = sizeof(T) == 4;
+    a.cuts = 1;
+    a.per = 1 << 30;
     auto launch = [&](auto kernel, int columns, int rows) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.N + columns - 1) / columns), (unsigned)((a.M + rows - 1) / rows)), block, 0, s, a);
+        const dim3 grid((unsigned)((a.N + columns - 1) / columns), (unsigned)((a.M + rows - 1) / rows), (unsigned)a.cuts);
+        hipLaunchKernelGGL(kernel, grid, dim3(FEW_WAVES * 64), 0, s, a);
     };
-    if (a.M <= 4 && few_columns<T>(a)) {
+    if (few_columns(f32, GATED, a.M, a.N, a.K)) {
         launch(dense_few_rows_kernel<T, ODD, GATED, 1, 4>, 4, 16);
-    } else {
-        const int blocks = a.M <= 16 ? 1 : few_blocks(sizeof(T) == 4, GATED, a.M, a.N, a.K).blocks;
-        if (blocks == 1) launch(dense_few_rows_kernel<T, ODD, GATED, 1, 16>, 16, 16);
-        else if (blocks == 2) launch(dense_few_rows_kernel<T, ODD, GATED, 2, 16>, 16, 32);
-        else launch(dense_few_rows_kernel<T, ODD, GATED, 4, 16>, 16, 64);
+        return hipGetLastError();
+    }
+    const FewBlocks plan = few_blocks(f32, GATED, a.M, a.N, a.K);
+    if (plan.cuts > 1) {
+        if (a.pieces == nullptr || a.piece_bytes < dense_few_rows_piece_bytes(f32, GATED, a.M, a.N, a.K)) return hipErrorInvalidValue;
+        a.cuts = plan.cuts;
+        a.per = plan.per;
+    }
+    if (plan.blocks == 1) launch(dense_few_rows_kernel<T, ODD, GATED, 1, 16>, 16, 16);
+    else if (plan.blocks == 2) launch(dense_few_rows_kernel<T, ODD, GATED, 2, 16>, 16, 32);
+    else launch(dense_few_rows_kernel<T, ODD, GATED, 4, 16>, 16, 64);
+    if (a.cuts > 1) {   // (few workgroups, so few elements: their quads are counted in 31 bits)
+        const long row = (a.N + 3) / 4;
+        hipLaunchKernelGGL((dense_few_sum_kernel<T, GATED>), dim3((unsigned)((a.M * row + 255) / 256)), dim3(256), 0, s, a, make_fastdiv((uint32_t)row));
     }
     return hipGetLastError();
 }

@@ -817,3 +817,12 @@ def test_calls_replayed_from_a_graph_between_eager_ones(kind, n, ic, oc):
 @pytest.mark.parametrize("in_place", [False, True])
 def test_residual_of_large_tiles(kind, size, in_place):
     check_forward(kind, *size, act=D.ACT_SILU, residual=True, in_place=in_place)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [5, 16, 33, 107])
+@pytest.mark.parametrize("ic,oc", [(8192, 100), (6001, 65), (3100, 1001), (2048, 3)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_long_sums_of_few_rows(kind, n, ic, oc, pad):
+    check_forward(kind, n, ic, oc, act=D.ACT_GELU, residual=True, save=True, pad=pad, in_place=pad == 0)
+    check_gated(kind, n, ic, oc, pad=pad)
