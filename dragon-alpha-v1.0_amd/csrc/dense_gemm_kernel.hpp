@@ -25,8 +25,9 @@ namespace alpha {
 static __device__ __forceinline__ void load_to_lds(unsigned lds, unsigned voffset, uintx4 rsrc)
 {
     // no register is written and nothing of the compiler's waits on it: the kernel's own s_waitcnt does (m0 is reserved to
-    // single instructions' use on this target, so nothing of the compiler's lives in it across this)
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc) : "memory");
+    // single instructions' use on this target, so nothing of the compiler's lives in it across this). A load into LDS may
+    // read m0 one wait state after a scalar write of it at the earliest, which the compiler keeps for its own instructions only.
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc) : "memory");
 }
 
 static __device__ __forceinline__ uintx4 make_rsrc(const void *p, unsigned bytes)   // bytes < 2^31: lanes that must read zeros ask for 2^31
