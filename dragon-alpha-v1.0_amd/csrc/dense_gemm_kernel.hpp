@@ -8,8 +8,8 @@
 // tiles are [rows][32 k] of 64-byte rows whose four 16-byte chunks are permuted by the row, so the 16 lanes that LDS serves
 // in a cycle (eight rows, two chunks each) touch different banks; T tiles are [32 k][rows] and are read by the transposing
 // LDS load, four k of 16 rows per instruction, their 32-byte pieces permuted by k.
-// Rows beyond the operand read zeros (the buffer descriptor ends with the last row's last 16-byte chunk: rows are whole
-// chunks long, zeros after their last element); k beyond K reads zeros too.
+// Rows beyond the operand read zeros (the buffer descriptor ends with the last row's last 16-byte chunk of the step, dense_bounds.hpp:
+// rows are whole chunks long, zeros after their last element); k beyond K reads zeros too.
 // The MFMA's rows are n and its columns m, so a lane holds four consecutive n of one m. A finished tile goes through LDS
 // (each wavefront its own part) so that every lane then has eight consecutive columns and a row leaves as one run of 128
 // bytes: stored from the registers as they are, 4096 x 4096 of bf16 took 17 us to write, this way 10.
@@ -18,6 +18,7 @@
 // clock (the same product of zeros runs at 1776 TF). With bias, SiLU and a residual (8192 x 8192 x 4096) 442 us. 1 % of the LDS
 // cycles are bank conflicts.
 #pragma once
+#include "dense_bounds.hpp"
 #include "dense_tile.hpp"
 
 namespace alpha {
@@ -103,10 +104,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
     const __bf16 *const A0 = static_cast<const __bf16 *>(a.A[0]), *const B0 = static_cast<const __bf16 *>(a.B[0]);
     const __bf16 *pA = A0 + atA + t0 / a.sources * stepA, *pB = B0 + atB + t0 / a.sources * stepB;   // in the first source
     const long toA1 = static_cast<const __bf16 *>(a.A[1]) - A0, toB1 = static_cast<const __bf16 *>(a.B[1]) - B0;
-    // bytes from a tile's first element to its end: straight, its rows' last chunk; T, of one k row
     const int spanN = GATED ? BN / 2 : BN;
-    const unsigned endA = AT ? (unsigned)((a.M - m0 + 7) & ~7) * 2 : (unsigned)(((long)((a.M - m0 < BM ? a.M - m0 : BM) - 1) * a.ldA + 32) * 2);
-    const unsigned endB = BT ? (unsigned)((a.N - n0 + 7) & ~7) * 2 : (unsigned)(((long)((a.N - n0 < spanN ? a.N - n0 : spanN) - 1) * a.ldB + 32) * 2);
+    const int rowsA = a.M - m0 < BM ? a.M - m0 : BM, rowsB = a.N - n0 < spanN ? a.N - n0 : spanN;
 
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
     uintx4 rA, rB;
@@ -124,12 +123,10 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_kernel(const Dense
             }
             if (GATED && (wave & 2)) qB += toB1;
         } else if (part == 1) {
-            const int rows = krem < 32 ? krem : 32;
-            rA = make_rsrc(qA, !AT ? endA : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldA * 2) + endA : 0u);
+            rA = make_rsrc(qA, AT ? tile_end_t(a.M - m0, (unsigned)a.ldA, krem) : tile_end_straight(rowsA, (unsigned)a.ldA, krem));
             inA = AT || kchunkA < krem;   // a straight row goes on into the next one
         } else if (part == 2) {
-            const int rows = krem < 32 ? krem : 32;
-            rB = make_rsrc(qB, !BT ? endB : rows > 0 ? (unsigned)(rows - 1) * (unsigned)(a.ldB * 2) + endB : 0u);
+            rB = make_rsrc(qB, BT ? tile_end_t(a.N - n0, (unsigned)a.ldB, krem) : tile_end_straight(rowsB, (unsigned)a.ldB, krem));
             inB = BT || kchunkB < krem;
         } else {
             lds = __builtin_amdgcn_readfirstlane(lds0 + stage + wave * 1024);
