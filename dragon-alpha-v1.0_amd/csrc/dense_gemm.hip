@@ -8,7 +8,7 @@ namespace alpha {
 // Adds the pieces of the cut tiles in their order and applies the epilogue: eight columns a thread, a workgroup 256 / (BN / 8)
 // rows of a tile (gated: BN / 16 threads a row, eight columns of each filter).
 template <typename T, bool GATED, bool FULL>
-__global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a, int bm, int bn, long a_row, long a_k, long b_row, long b_k)
+__global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a, int bm, int bn)
 {
     const int lanes = bn / (GATED ? 16 : 8), rows = 256 / lanes, per_tile = bm / rows;
     const int cut = (int)blockIdx.x / per_tile, row = (int)blockIdx.x % per_tile * rows + (int)threadIdx.x / lanes, lane = (int)threadIdx.x % lanes;
@@ -33,16 +33,6 @@ __global__ __launch_bounds__(256) void dense_pieces_kernel(const DenseTileArgs a
             run_load(src + 32, t);
 #pragma unroll
             for (int e = 0; e < 8; e++) u[e] += t[e];
-        }
-    }
-    if constexpr (__is_same(T, float)) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if (n + e >= a.N) break;
-            if (v[e] != v[e])
-                v[e] = dense_element(a.A[0], a.A[1], m * a_row, a_k, a.B[0], a.B[1], (n + e) * b_row, b_k, GATED ? 1 : a.sources, a.K);
-            if (GATED && u[e] != u[e])
-                u[e] = dense_element(a.A[0], a.A[0], m * a_row, a_k, a.B[1], a.B[1], (n + e) * b_row, b_k, 1, a.K);
         }
     }
     if (a.ep.vec && n + 8 <= a.N) {
@@ -160,8 +150,7 @@ hipError_t launch_dense_product(hipStream_t s, const DenseProduct &p)
     const int bm = DENSE_TILE_M[plan.tile], bn = DENSE_TILE_N[plan.tile], cut = plan.tiles_m * plan.tiles_n - plan.whole;
     if (e != hipSuccess || cut == 0) return e;
     const dim3 grid((unsigned)cut * (unsigned)(bm * bn / (p.gated ? 16 : 8) / 256));
-    const long a_row = p.a_t ? 1 : p.A.ld, a_k = p.a_t ? p.A.ld : 1, b_row = p.b_t ? 1 : p.B.ld, b_k = p.b_t ? p.B.ld : 1;
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, bm, bn, a_row, a_k, b_row, b_k); };
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, bm, bn); };
     if (p.gated) p.f32 ? launch(dense_pieces_kernel<float, true, true>) : launch(dense_pieces_kernel<__bf16, true, true>);
     else if (p.b_t) p.f32 ? launch(dense_pieces_kernel<float, false, false>) : launch(dense_pieces_kernel<__bf16, false, false>);
     else p.f32 ? launch(dense_pieces_kernel<float, false, true>) : launch(dense_pieces_kernel<__bf16, false, true>);

@@ -15,8 +15,8 @@
 //     barrier: every read of this step's planes and every write of the next step's is done
 //     run 3: l h', m h', h h'  reads the next step's l', h
 // so the one barrier of a step (256 x 128: 192 MFMAs per SIMD) stands between MFMAs whose operands are in registers.
-// An infinity or NaN makes NaN (h - h), and so does a value that rounds up beyond bf16's range: a NaN result is computed again
-// in plain fp32 (dense_element).
+// An infinity or NaN makes NaN (h - h), and so does a value that rounds up beyond bf16's range; products of parts may overflow
+// where the whole does not. What is not finite at the end is computed once more in plain fp32 (plain_rows).
 #pragma once
 #include "dense_tile.hpp"
 
@@ -254,7 +254,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void dense_tile_f32_kernel(const D
         step(ah1, bl1, ah0, bl0);
     }
     lds_barrier();   // every read of the tiles is done
-    tile_out<float, AT, BT, GATED, BM, BN, WM, WN, 2 * (int)BUFFER>(a, acc, smem, lane, wave, wm, wn, m0, n0, cut, piece, tile - a.whole, cut_tiles);
+    const int k_first = t0 / a.sources * 32, k_end = k_first + left / a.sources * 32;
+    tile_out<float, AT, BT, GATED, BM, BN, WM, WN, 2 * (int)BUFFER>(a, acc, smem, lane, wave, wm, wn, m0, n0, cut, piece, tile - a.whole, cut_tiles, k_first,
+                                                                    k_end < a.K ? k_end : a.K);
 }
 
 }  // namespace alpha

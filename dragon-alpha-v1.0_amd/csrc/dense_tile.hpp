@@ -1,5 +1,5 @@
-// What the dense tile kernels share: their arguments, the order of the tiles, the bank permutations of their LDS tiles, how
-// a finished tile leaves, and the element that is computed once more.
+// What the dense tile kernels share: their arguments, the order of the tiles, the bank permutations of their LDS tiles and how
+// a finished tile leaves.
 #pragma once
 #include "dense_finish.hpp"
 
@@ -64,21 +64,75 @@ static __device__ __forceinline__ int t_permutation(int k) { return ((k & 3) | (
 // four groups of rows must come to four different chunks: 0, 3, 2, 1 for g = 0 .. 3. Counted: no conflicts.
 static __device__ __forceinline__ int s_permutation(int g) { return (g & 1) | ((g ^ (g >> 1)) & 1) << 1; }
 
+static __device__ __forceinline__ bool finite_sum(float v) { return fabsf(v) <= 3.40282347e38f; }
 
-// One fp32 element of C once more as a plain chain of fused multiply-adds: taken where the sum of the products of parts is NaN,
-// which it also is where an operand is infinite (or within 2^-9 of the end of the range). Ends at the first NaN.
-static __device__ __attribute__((noinline)) float dense_element(const void *A0, const void *A1, long a_row, long a_k, const void *B0, const void *B1,
-                                                                long b_row, long b_k, int sources, int K)
+// fp32: 16 rows of C (from m0 on, 64 columns from n0 on, at `part` in LDS) whose sums are not all finite, once more as plain fp32
+// products over the workgroup's reduction (cut tiles: its piece of it), on v_mfma_f32_16x16x4_f32 with operands straight from memory; what is
+// finite stays the sum of the parts. 16 k a turn, the lane's being k + 4 (lane / 16) + s in the s-th MFMA. What lies beyond M, N or
+// K is not read (the last row, column or k again), and what is beyond M or N not looked at. All wavefronts and pieces work side by
+// side, none longer than its own part of the product: 12544 x 256 -> 1024 forward 62 us, with one infinity in X 76, all of X infinite
+// 198; its backward 104, 251 and 357.
+template <bool AT, bool BT, bool GATED>
+static __device__ __forceinline__ void plain_rows(const DenseTileArgs &a, float *part, int row_floats, int lane, int m0, int n0, int k_first, int k_end)
 {
-    float acc = 0.f;
-    for (int s = 0; s < sources; s++) {
-        const float *a = static_cast<const float *>(s ? A1 : A0) + a_row, *b = static_cast<const float *>(s ? B1 : B0) + b_row;
-        for (int k = 0; k < K; k++, a += a_k, b += b_k) {
-            acc = fmaf(*a, *b, acc);
-            if (acc != acc) return acc;
-        }
+    const int l16 = lane & 15, q = lane >> 4, m = m0 + l16;
+    float *const mine = part + l16 * row_floats + q * 4;      // + 16 j: four columns of fragment j
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const floatx4 v = *reinterpret_cast<const floatx4 *>(mine + 16 * j);
+        const int n = n0 + 16 * (GATED ? j & 1 : j) + 4 * q;
+#pragma unroll
+        for (int e = 0; e < 4; e++) any |= m < a.M && n + e < a.N && !finite_sum(v[e]);
     }
-    return acc;
+    if (__ballot(any) == 0) return;     // uniform
+    const long row = (m < a.M ? m : a.M - 1) * (AT ? 1 : a.ldA);
+    long col[4];
+    floatx4 c[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int n = n0 + 16 * (GATED ? j & 1 : j) + l16;
+        col[j] = (n < a.N ? n : a.N - 1) * (BT ? 1 : a.ldB);
+        c[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll 1
+    for (int source = 0; source < (GATED ? 1 : a.sources); source++) {
+        const float *A = static_cast<const float *>(source ? a.A[1] : a.A[0]) + row;
+        const float *B0 = static_cast<const float *>(source ? a.B[1] : a.B[0]), *B1 = GATED ? static_cast<const float *>(a.B[1]) : B0;
+        // four consecutive k of a row or column: 16 bytes, or four rows
+        auto load = [&](auto whole, const float *p, long ld, int k, float (&v)[4]) __attribute__((always_inline)) {
+            if (whole && ld == 1) {
+                __builtin_memcpy(v, p + k, 16);
+                return;
+            }
+#pragma unroll
+            for (int s = 0; s < 4; s++) v[s] = p[(whole || k + s < k_end ? k + s : k_end - 1) * ld];
+        };
+        auto turn = [&](auto whole, int k) __attribute__((always_inline)) {
+            float x[4], w[4][4];
+            load(whole, A, AT ? a.ldA : 1, k, x);
+#pragma unroll
+            for (int j = 0; j < 4; j++) load(whole, (GATED && j >= 2 ? B1 : B0) + col[j], BT ? a.ldB : 1, k, w[j]);
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const bool there = whole || k + s < k_end;
+#pragma unroll
+                for (int j = 0; j < 4; j++) c[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(there ? w[j][s] : 0.f, there ? x[s] : 0.f, c[j], 0, 0, 0);
+            }
+        };
+        int k0 = k_first;
+#pragma unroll 1
+        for (; k0 + 16 <= k_end; k0 += 16) turn(std::true_type{}, k0 + 4 * q);
+        if (k0 < k_end) turn(std::false_type{}, k0 + 4 * q);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        floatx4 *const to = reinterpret_cast<floatx4 *>(mine + 16 * j);
+        floatx4 v = *to;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = finite_sum(v[e]) ? v[e] : c[j][e];
+        *to = v;
+    }
 }
 
 // A finished tile leaves two fragment rows (32 rows of C) at a time through the wavefront's part of LDS, so that a lane then has
@@ -87,7 +141,8 @@ static __device__ __attribute__((noinline)) float dense_element(const void *A0, 
 // of the tile. Every wavefront is done with the tiles in LDS.
 template <typename T, bool AT, bool BT, bool GATED, int BM, int BN, int WM, int WN, int LDS>
 static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const floatx4 (&acc)[BM / WM / 16][BN / WN / 16], char *smem, int lane, int wave, int wm,
-                                                int wn, int m0, int n0, bool cut, int piece, int cut_tile, int cut_tiles)
+                                                int wn, int m0, int n0, bool cut, int piece, int cut_tile, int cut_tiles, int k_first = 0,
+                                                int k_end = 0)
 {
     constexpr int TM = BM / WM, TN = BN / WN, MF = TM / 16;
     constexpr bool FULL = !BT;     // B with k as its rows: a backward's product
@@ -103,7 +158,18 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
     // The turns over pairs of fragment rows are not unrolled (only their copies out of the registers are): a workgroup runs
     // this once, and what it costs is largely the fetching of its code.
     const bool vec = a.ep.vec;
-    unsigned again = 0;   // fp32: runs with a NaN among them, computed once more below
+    // fp32: an operand that is infinite or NaN (or within 2^-9 of the end of the range) makes NaN of the products of its parts
+    bool again = false;
+    if constexpr (__is_same(T, float)) {
+        float check = 0.f;     // NaN as soon as one of the sums is not finite
+#pragma unroll
+        for (int i = 0; i < MF; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) check = fmaf(acc[i][j][e], 0.f, check);
+        again = __ballot(check != check) != 0;
+    }
 #pragma unroll 1
     for (int i = 0; i < MF; i += 2) {
         for_each<MF / 2>([&](auto pair) __attribute__((always_inline)) {
@@ -114,6 +180,13 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
                     for (int j = 0; j < 4; j++) *reinterpret_cast<floatx4 *>(part + (h * 16 + l16) * ROW + j * 16 + q * 4) = acc[2 * pair + h][j];
             }
         });
+        if constexpr (__is_same(T, float)) {
+            if (again) {   // uniform; a lane reads and writes what it wrote itself
+#pragma unroll 1
+                for (int h = 0; h < 2; h++)
+                    plain_rows<AT, BT, GATED>(a, part + h * 16 * ROW, ROW, lane, m0 + wm * TM + (i + h) * 16, n0 + wn * (GATED ? 32 : 64), k_first, k_end);
+            }
+        }
         wave_fence();
         // One turn: AT_ONCE rows. AHEAD: a large tile's residual is loaded for all turns first, or each
         // would wait for its own (8192 x 1024 x 4096 of bf16 with a residual 104 -> 96 us).
@@ -142,15 +215,6 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
                 if constexpr (GATED) run_store(dst + 32, u);
                 return;
             }
-            if constexpr (__is_same(T, float)) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; e++) sum += GATED ? v[e] + u[e] : v[e];
-                if (sum != sum) {   // (also where infinities of both signs meet: no harm)
-                    again |= 1u << (i / 2 * TURNS + y / AT_ONCE);
-                    return;
-                }
-            }
             if (vec && n + 8 <= a.N) {
                 if constexpr (GATED) dense_finish_gated<T, 8, true>(a.ep, v, u, m, n);
                 else dense_finish<T, 8, FULL, true>(a.ep, v, m, n, 8, residual);
@@ -167,27 +231,6 @@ static __device__ __forceinline__ void tile_out(const DenseTileArgs &a, const fl
             for (int y = 0; y < 32; y += AT_ONCE) turn(y, nullptr);
         }
         wave_fence();
-    }
-    if constexpr (__is_same(T, float)) {
-        static_assert(MF / 2 * TURNS <= 32, "one bit per run");
-#pragma unroll 1
-        while (again) {
-            const int bit = __ffs(again) - 1;
-            again &= again - 1;
-            const long m = m0 + wm * TM + bit / TURNS * 32 + bit % TURNS * AT_ONCE + lane / LANES;
-#pragma unroll 1
-            for (int e = 0; e < 8 && n + e < a.N; e++) {
-                float x[1], z[1] = {0.f};
-                x[0] = dense_element(a.A[0], a.A[1], AT ? m : m * a.ldA, AT ? a.ldA : 1, a.B[0], a.B[1], BT ? n + e : (n + e) * a.ldB,
-                                     BT ? a.ldB : 1, GATED ? 1 : a.sources, a.K);
-                if constexpr (GATED) {
-                    z[0] = dense_element(a.A[0], a.A[0], m * a.ldA, 1, a.B[1], a.B[1], (n + e) * a.ldB, 1, 1, a.K);
-                    dense_finish_gated<T, 1, false>(a.ep, x, z, m, n + e);
-                } else {
-                    dense_finish<T, 1, FULL, false>(a.ep, x, m, n + e);
-                }
-            }
-        }
     }
 }
 

@@ -25,7 +25,7 @@
  *   - Outputs must not overlap inputs, the workspace or each other, except where said.
  *   - Large fp32 products run on the bf16 matrix pipe as sums of exact three-part splits (24 bits): six of the nine partial
  *     products, the left-out ones together below 2^-23 of a product. Others are plain fp32. Infinities and NaN come out as in
- *     plain fp32 either way.
+ *     plain fp32 either way; what is not finite is computed again, so a product that is full of them takes three to four times as long.
  *
  * Return value: 0 on success, a hipError_t value, or ALPHA_DENSE_EINVAL; alpha_dense_last_error() has the thread's message.
  */
