@@ -1,5 +1,6 @@
 // The dense product's tile kernel for fp32: C[m, n] = sum_k A(m, k) B(n, k) on the bf16 matrix pipe, sixteen times the rate of
-// the fp32 one. x = h + m + l exactly, three bf16 of 8 significant bits each (rounded to nearest, signs of their own); of the
+// the fp32 one. x = h + m + l exactly, three bf16 of 8 significant bits each (rounded to nearest, signs of their own; |x| < 2^-110
+// to within half of bf16's last subnormal, 2^-134, which the matrix pipe takes as they are); of the
 // nine products of parts the six above 2^-24 of the whole are summed, small ones first, in fp32:
 //     x y = h l' + m m' + h m' + l h' + m h' + h h'   (left out: m l', l m', l l', together below 2^-23 |x y|).
 // 2.5 PF / 6 = 417 TF bound, 157 TF through v_mfma_f32_16x16x4_f32. Measured: 4096 x 1024 x 4096 with GELU and both outputs 185 us,

@@ -23,8 +23,9 @@
  *   - `streams`, `length`: as in alpha_conv.h; everything is enqueued on streams[0], which belongs to the current device,
  *     as does the memory. Calls may be captured into a graph. Results are bit-identical from run to run.
  *   - Outputs must not overlap inputs, the workspace or each other, except where said.
- *   - Large fp32 products run on the bf16 matrix pipe as sums of exact three-part splits (24 bits): six of the nine partial
- *     products, the left-out ones together below 2^-23 of a product. Others are plain fp32. Infinities and NaN come out as in
+ *   - Large fp32 products run on the bf16 matrix pipe as sums of three-part splits: six of the nine partial products, the left-out
+ *     ones together below 2^-23 of a product. The split keeps all 24 bits of an operand of 2^-110 and more; of a smaller one, whose
+ *     last parts would be below bf16's last subnormal, it keeps what is above 2^-134. Others are plain fp32. Infinities and NaN come out as in
  *     plain fp32 either way; what is not finite is computed again, so a product that is full of them takes three to four times as long.
  *
  * Return value: 0 on success, a hipError_t value, or ALPHA_DENSE_EINVAL; alpha_dense_last_error() has the thread's message.

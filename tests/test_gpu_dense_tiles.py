@@ -151,6 +151,19 @@ def test_fp32_tile_products_with_an_identity_are_exact(n, ic):
     assert torch.equal(y, x.t())
 
 
+@pytest.mark.parametrize("exponent", [-100, -109, -110, -111, -113, -116, -120, -126])
+def test_fp32_tile_products_of_small_operands(exponent):
+    """All bits of an operand of 2^-110 and more; below, what is left of it behind three bf16 parts is at most half of the last
+    subnormal, 2^-134. (The other operand is a power of two, so the product adds nothing.)"""
+    n, ic = 4097, 1003
+    must_take("f32", "forward", n, ic, ic, ("ss", 128, 128, True))
+    x = matrix(n, ic, torch.float32, 9)
+    x = (1 + x.abs().clamp(max=0.999)) * 2.0 ** exponent
+    y, _ = run_forward("f32", x, torch.eye(ic, device="cuda") * 2.0 ** 100, None, 0, None, False)
+    off = (y.double() * 2.0 ** -100 - x.double()).abs().max()
+    assert float(off) <= (0.0 if exponent >= -110 else 2.0 ** -134)
+
+
 # ---- rows beyond 32 bits ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", TYPES)
 def test_rows_of_the_largest_stride(kind):
