@@ -49,3 +49,42 @@ def test_gelu(kind, lo, hi):
 @pytest.mark.parametrize("lo,hi", [(-12, -8), (-8, -6), (-6, -5), (-5, -4), (-4, -2), (-0.5, 4), (4, 12), (12, 100)])
 def test_gelu_derivative(kind, lo, hi):
     check(kind, D.ACT_GELU, lo, hi, 4, True)      # (it is 0 at -0.75)
+
+
+SIGMOID_RANGES = [(-85, -17), (-17, -8), (-8, -2), (-2, -1e-3), (1e-3, 4), (4, 10), (10, 17), (17, 85)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lo,hi", SIGMOID_RANGES)
+@pytest.mark.parametrize("act", [D.ACT_SILU, D.ACT_SIGMOID])
+def test_silu_and_sigmoid(kind, act, lo, hi):
+    check(kind, act, lo, hi, 1, False)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lo,hi", SIGMOID_RANGES)
+def test_sigmoid_derivative(kind, lo, hi):
+    check(kind, D.ACT_SIGMOID, lo, hi, 1, True)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lo,hi", [(-85, -17), (-17, -8), (-8, -2), (-1, -1e-3), (1e-3, 4), (4, 10), (10, 17), (17, 85)])
+def test_silu_derivative(kind, lo, hi):
+    check(kind, D.ACT_SILU, lo, hi, 4, True)      # (it is 0 at -1.28)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("act", [D.ACT_GELU, D.ACT_SILU, D.ACT_SIGMOID])
+def test_far_values(kind, act):
+    """Where the exponential is 0 or would overflow: the limits, no NaN; of infinities and NaN what the formula has."""
+    dtype = TYPES[kind][1]
+    z = torch.tensor([-3e38, -1e20, -1e4, -200.0, 200.0, 1e4, 1e20, 3e38, float("inf"), float("nan")] + [0.0] * 54, device="cuda").to(dtype).view(-1, 1)
+    one = torch.ones(1, 1, dtype=dtype, device="cuda")
+    y, _ = run_forward(kind, z, one, None, act, None, False)
+    low, high = y[:4].float(), y[4:9].float()
+    assert bool((low.abs() < 1e-30).all()) and bool(torch.isnan(y[9, 0]))
+    assert torch.equal(high, torch.ones_like(high) if act == D.ACT_SIGMOID else z[4:9].float())
+    assert float(y[10]) == (0.5 if act == D.ACT_SIGMOID else 0.0)
+    d = run_backward(kind, torch.ones_like(z[:8]).contiguous(), z[:8].contiguous(), act, z[:8].contiguous(), one, ("db", "dx"))["dx"].float()
+    assert bool((d[:4].abs() < 1e-30).all())
+    assert torch.equal(d[4:], torch.zeros_like(d[4:]) if act == D.ACT_SIGMOID else torch.ones_like(d[4:]))
