@@ -41,13 +41,20 @@ def _bind():
     return _functions
 
 
-def _array(kind, values):
-    return None if values is None else (kind * max(1, len(values)))(*values)
+def _array(kind, values, count=0):
+    """A host array for the C side, which reads `count` entries."""
+    if values is None:
+        return None
+    if len(values) < count:
+        raise native.AlphaConvError("a list of %d entries is shorter than the count %d" % (len(values), count))
+    return (kind * max(1, len(values)))(*values)
 
 
-def _call(name, streams, *args):
+def _call(name, streams, length, *args):
     """`args` as ctypes takes them for the signature: integers, floats, arrays."""
-    rc = (_functions or _bind())[name](_ONE(streams[0]) if len(streams) == 1 else (_L * max(1, len(streams)))(*streams), *args)
+    if len(streams) < length:
+        raise native.AlphaConvError("%s: %d streams given, length %d" % (name, len(streams), length))
+    rc = (_functions or _bind())[name](_ONE(streams[0]) if len(streams) == 1 else (_L * max(1, len(streams)))(*streams), length, *args)
     if rc != 0:
         raise native.AlphaConvError("%s failed (%d): %s" % (name, rc, _functions["alpha_dense_last_error"]().decode()))
 
@@ -114,10 +121,10 @@ class Cuda_dense:
 
     @staticmethod
     def gradClip_workspace(count, lengths):
-        return _workspace("alpha_gradClip_workspace", count, _array(_L, lengths))
+        return _workspace("alpha_gradClip_workspace", count, _array(_L, lengths, count))
 
     @staticmethod
     def gradClip(streamArray, length, count, types, lengths, src, dst, max_norm, eps, norm_c, workspace, workspace_bytes):
         """norm_c = {norm, c} with c = min(1, max_norm / (norm + eps)); dst = src * c (dst None: only the norm)."""
-        _call("alpha_gradClip", streamArray, length, count, _array(_I, types), _array(_L, lengths), _array(_P, src), _array(_P, dst),
-              max_norm, eps, norm_c, workspace, workspace_bytes)
+        _call("alpha_gradClip", streamArray, length, count, _array(_I, types, count), _array(_L, lengths, count), _array(_P, src, count),
+              _array(_P, dst, count), max_norm, eps, norm_c, workspace, workspace_bytes)
