@@ -107,6 +107,32 @@ int check_distinct(const char *fn, const void *const *outputs, int n_out, const 
     return 0;
 }
 
+// Clipping: a tensor written twice would be scaled twice, or by two workgroups at a time; one that is another's source, before or
+// after it is read. A filter of 2^17 bits (16 KB on the stack) leaves few addresses to look for one by one.
+int check_clip_lists(const char *fn, int count, const int64_t *lengths, const void *const *src, void *const *dst)
+{
+    uint64_t seen[2048] = {};
+    auto place = [](const void *p) { return (unsigned)((reinterpret_cast<uintptr_t>(p) * 0x9e3779b97f4a7c15ull) >> 47); };
+    auto look = [&](const void *p, int end, int except) {
+        if ((seen[place(p) >> 6] >> (place(p) & 63) & 1) == 0) return -1;
+        for (int j = 0; j < end; j++)
+            if (j != except && lengths[j] > 0 && dst[j] == p) return j;
+        return -1;
+    };
+    for (int i = 0; i < count; i++) {
+        if (lengths[i] == 0) continue;
+        const int j = look(dst[i], i, i);
+        if (j >= 0) return fail("%s: dst[%d] and dst[%d] share an address", fn, j, i);
+        seen[place(dst[i]) >> 6] |= 1ull << (place(dst[i]) & 63);
+    }
+    for (int i = 0; i < count; i++) {
+        if (lengths[i] == 0 || src[i] == dst[i]) continue;
+        const int j = look(src[i], count, i);
+        if (j >= 0) return fail("%s: dst[%d] shares its address with src[%d]", fn, j, i);
+    }
+    return 0;
+}
+
 #define TRY(call)             \
     do {                      \
         if (int rc_ = (call)) \
@@ -571,6 +597,7 @@ ALPHA_EXPORT int alpha_gradClip(const int64_t *streams, int length, int count, c
         if (dst != nullptr && (dst[i] == nullptr || (reinterpret_cast<uintptr_t>(dst[i]) & (size_of(types[i]) - 1))))
             return fail("%s: dst[%d] is null or not aligned to its element", fn, i);
     }
+    if (dst != nullptr) TRY(check_clip_lists(fn, count, lengths, src, dst));
     hipStream_t s = reinterpret_cast<hipStream_t>((intptr_t)streams[0]);
     TRY(check_device(fn, s));
     return hip_status(launch_grad_clip(s, count, types, lengths, src, dst, max_norm, eps, norm_c, static_cast<double *>(workspace)), fn);

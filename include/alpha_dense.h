@@ -98,8 +98,8 @@ int alpha_dgatedMatMul(const int64_t *streams, int length, int type,
 /* The global norm of `count` gradients and clipping by it:
  *     norm = sqrt(sum over all tensors and elements of g^2),  c = min(1, max_norm / (norm + eps)),  dst = g * c.
  * types[i], lengths[i] (elements, >= 0), src[i], dst[i]: HOST arrays, read during the call; the tensors are dense device
- * memory aligned to their element, dst[i] of src[i]'s type, and dst[i] may be src[i] (in place). dst may be NULL: only the
- * norm. norm_c: two device floats, {norm, c}, written; NaN and infinities follow the formula (a NaN makes c NaN; an
+ * memory aligned to their element, dst[i] of src[i]'s type, and dst[i] may be src[i] (in place) but no other src or dst: the same gradient
+ * twice is refused where it would be scaled twice. dst may be NULL: only the norm. norm_c: two device floats, {norm, c}, written; NaN and infinities follow the formula (a NaN makes c NaN; an
  * infinite norm makes c 0 and the infinite elements NaN), so a caller sees them in norm_c[0]. max_norm and eps are finite and >= 0, max_norm + eps > 0. */
 int64_t alpha_gradClip_workspace(int count, const int64_t *lengths);
 int alpha_gradClip(const int64_t *streams, int length, int count, const int *types, const int64_t *lengths,
