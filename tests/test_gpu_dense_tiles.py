@@ -307,6 +307,24 @@ def test_gated_backward_tiles_with_infinities_and_nans(case):
         same_pattern(got[name], d.sum(0, keepdim=True), (name, case))
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,ic,oc", [(1, 40, 56), (5, 9, 33), (70, 137, 73), (300, 33, 9), (2, 5, 4099), (4416, 33, 35), (2319, 2465, 521)])
+@pytest.mark.parametrize("act", [D.ACT_NONE, D.ACT_LEAKY_RELU])
+def test_backward_of_any_form_with_infinities_and_nans(kind, n, ic, oc, act):
+    """Small products straight from memory, long sums cut over workgroups, bf16 tiles."""
+    dtype = TYPES[kind][1]
+    x, w, dy = matrix(n, ic, dtype, 1, pad=3), matrix(oc, ic, dtype, 2, 0.1, pad=1), matrix(n, oc, dtype, 3, pad=5)
+    z = matrix(n, oc, dtype, 4) if act != D.ACT_NONE else None
+    dy[n // 2, oc // 3], dy[n - 1, oc - 1], dy[n // 3, 0] = INF, -INF, NAN
+    x[n // 2, ic // 2], x[n - 1, ic - 1] = 0.0, INF
+    w[oc // 3, ic // 3], w[oc // 2, 0], w[oc - 1, ic - 1] = 0.0, -INF, INF
+    got = run_backward(kind, dy, z, act, x, w)
+    dz = dy.double() if z is None else dy.double() * slope64(act, z.double())
+    same_pattern(got["dx"], dz @ w.double(), "dx")
+    same_pattern(got["dw"], dz.t() @ x.double(), "dw")
+    same_pattern(got["db"], dz.sum(0, keepdim=True), "db")
+
+
 def _us(call):
     times = []
     for _ in range(5):
