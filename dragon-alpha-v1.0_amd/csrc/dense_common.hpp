@@ -11,7 +11,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 // ---- activations ---------------------------------------------------------------------------------------------------
-// exp(-z) from the hardware's 2^x: z log2(e) as a rounded product and its remainder, the remainder applied to first order;
+// exp(z) from the hardware's 2^x: z log2(e) as a rounded product and its remainder, the remainder applied to first order;
 // within a few units of 2^-24, 2^x's own error among them.
 static __device__ __forceinline__ float dense_exp(float z)
 {
@@ -19,13 +19,13 @@ static __device__ __forceinline__ float dense_exp(float z)
     const float p = __builtin_amdgcn_exp2f(t);
     return fabsf(t) < 126.f ? fmaf(p, r * 0.69314718f, p) : p;   // (beyond: near 0 or infinity, and r may be no number)
 }
-// S(z) = 1 / (1 + exp(-z)) and, exactly as well, 1 - S(z) = S(-z): both from e = exp(-|z|), as 1 and e over 1 + e. (1 minus a rounded S
-// has nothing left from z = 17 on, where the derivative S(z) S(-z) still does.)
-static __device__ __forceinline__ float dense_sigmoid(float z, float &complement)
+// S(z) = 1 / (1 + exp(-z)); 1 / (1 + inf) = 0 from the hardware's reciprocal (2^-23).
+static __device__ __forceinline__ float dense_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + dense_exp(-z)); }
+// S(z) (1 - S(z)) = S(z) S(-z) = e / (1 + e)^2 with e = exp(-|z|). (1 minus a rounded S has nothing left from z = 17 on.)
+static __device__ __forceinline__ float dense_sigmoid_slope(float z)
 {
-    const float e = dense_exp(-fabsf(z)), larger = __builtin_amdgcn_rcpf(1.f + e), smaller = e * larger;
-    complement = z < 0.f ? larger : smaller;
-    return z < 0.f ? smaller : larger;
+    const float e = dense_exp(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e);
+    return e * r * r;
 }
 
 // P(z) = (1 + erf(z / sqrt 2)) / 2 and its derivative D(z) = exp(-z^2 / 2) / sqrt(2 pi), from one exponential. The tail P(-a), a = |z|,
@@ -58,12 +58,12 @@ static __device__ __forceinline__ float dense_normal(float z, float &density)
 template <typename T>
 static __device__ __forceinline__ float dense_act(int act, float z, float k)
 {
-    float other;
+    float density;
     switch (act) {   // uniform
     case ALPHA_DENSE_ACT_LEAKY_RELU: return z > 0.f ? z : z * k;
-    case ALPHA_DENSE_ACT_GELU: return z * dense_normal<T>(z, other);
-    case ALPHA_DENSE_ACT_SILU: return z * dense_sigmoid(z, other);
-    case ALPHA_DENSE_ACT_SIGMOID: return dense_sigmoid(z, other);
+    case ALPHA_DENSE_ACT_GELU: return z * dense_normal<T>(z, density);
+    case ALPHA_DENSE_ACT_SILU: return z * dense_sigmoid(z);
+    case ALPHA_DENSE_ACT_SIGMOID: return dense_sigmoid(z);
     default: return z;
     }
 }
@@ -79,14 +79,10 @@ static __device__ __forceinline__ float dense_act_slope(int act, float z, float 
         return fmaf(z, density, p);
     }
     case ALPHA_DENSE_ACT_SILU: {
-        float rest;
-        const float s = dense_sigmoid(z, rest);
-        return s * fmaf(z, rest, 1.f);
+        const float s = dense_sigmoid(z);
+        return s * fmaf(z, 1.f - s, 1.f);
     }
-    case ALPHA_DENSE_ACT_SIGMOID: {
-        float rest;
-        return dense_sigmoid(z, rest) * rest;
-    }
+    case ALPHA_DENSE_ACT_SIGMOID: return dense_sigmoid_slope(z);
     default: return 1.f;
     }
 }
