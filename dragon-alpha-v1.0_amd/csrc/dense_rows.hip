@@ -1,6 +1,9 @@
 // The passes around a dense product, each bound by memory: rows of bf16 that the tile kernel's 128-bit loads cannot take copied
-// to ones they can, and deltaZ = deltaY * act'(Z) with its column sums (fp32 SiLU 4992 x 2496 28 us, 5.3 TB/s; GELU 12544 x 1024 37 us,
-// 4.2 TB/s, by its erf; bf16 SiLU 8192 x 4096 47 us, 4.3 TB/s).
+// to ones they can, and deltaZ = deltaY * act'(Z) with its column sums (fp32 SiLU 4992 x 2496 28 us, 5.3 TB/s; GELU 12544 x 1024 36 us,
+// 4.3 TB/s; bf16 SiLU 8192 x 4096 47 us, 4.3 TB/s).
+// A bf16 call stores deltaZ in bf16, as the products' operand is on the matrix pipe: each element off by half a step, 2^-8 at most, so
+// deltaX and deltaW are off by 0.0023 of their rms instead of the 0.0017 that their own rounding leaves. Two bf16 parts would keep the
+// difference and double both products (410 of the 466 us of 8192 x 4096 -> 4096). The column sums are of the unrounded values.
 #include "dense_common.hpp"
 
 #include <algorithm>
@@ -89,7 +92,7 @@ constexpr int DELTA_ROWS = 4;
 template <typename T, bool GATED, int LANES, int ACT>
 __global__ __launch_bounds__(256) void dense_delta_kernel(const DenseDelta d, long rows_per)
 {
-    constexpr int ROWS = LANES == 1 ? 1 : sizeof(T) == 4 && ACT == ALPHA_DENSE_ACT_GELU ? 2 : DELTA_ROWS;   // (erf is long)
+    constexpr int ROWS = LANES == 1 ? 1 : DELTA_ROWS;
     constexpr int SIDE = 256 / LANES, COLS = LANES * 8;       // rows side by side, columns
     __shared__ float part[GATED ? 2 : 1][SIDE][COLS + 1];
     const int lane = threadIdx.x % LANES, ry = threadIdx.x / LANES, c = (blockIdx.x * LANES + lane) * 8;
