@@ -186,7 +186,7 @@ double dense_short_us(int f32, int gated, int M, int N, int K);
 hipError_t launch_dense_short(hipStream_t s, const DenseFewRows &a);
 hipError_t launch_dense_few_rows(hipStream_t s, const DenseFewRows &a);
 
-// Small products of a backward (B with k as its rows), operands as they are, no pieces (dense_small.hip).
+// Small products of a backward (B with k as its rows), operands as they are (dense_small.hip).
 size_t dense_small_piece_bytes(int f32, int M, int N, int K, int sources);
 bool dense_small_preferred(int f32, int a_t, int M, int N, int K, int sources);
 hipError_t launch_dense_small(hipStream_t s, const DenseProduct *px, const DenseProduct *pw);   // deltaX and deltaW, one may be null

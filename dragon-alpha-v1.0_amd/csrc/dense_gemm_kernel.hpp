@@ -15,7 +15,8 @@
 // bytes: stored from the registers as they are, 4096 x 4096 of bf16 took 17 us to write, this way 10.
 // Gated: of every 64 tile columns 32 are of one filter and 32, the same ones, of the other.
 // Measured: 8192 x 4096 x 8192 391 us, 1405 TF; the matrix pipe is busy 66 % of the cycles, at 1.6 GHz: the card's power limit sets the
-// clock (the same product of zeros runs at 1776 TF). With bias, SiLU and a residual (8192 x 8192 x 4096) 442 us. 1 % of the LDS
+// clock (the same product of zeros runs at 1776 TF). With bias, SiLU and a residual (8192 x 8192 x 4096) 455 us
+// (443 to 460 from card to card). 1 % of the LDS
 // cycles are bank conflicts.
 #pragma once
 #include "dense_bounds.hpp"

@@ -6,13 +6,14 @@
  *
  * Conventions:
  *   - Element types: ALPHA_DENSE_F32, ALPHA_DENSE_BF16; every tensor of a call has the call's type (gradClip: one type per
- *     tensor). Sums are held in fp32 (the norm's in fp64) and rounded once, to the output's type; bf16 backward rounds
- *     deltaZ (deltaG, deltaU) to bf16 before its products, deltaB is summed from the unrounded values.
+ *     tensor). Sums are held in fp32 (the norm's in fp64 from the sums of 16 bytes' squares on) and rounded once, to the output's
+ *     type; bf16 backward rounds deltaZ (deltaG, deltaU) to bf16, the matrix pipe's operand, before its products, deltaB is summed
+ *     from the unrounded values.
  *   - Matrices are row-major, X[N,IC], W[OC,IC] (a filter W[OC,1,1,IC]), Y[N,OC]; `*_stride` is the distance of two rows
  *     in elements (>= the row's length, <= 2^22). N < 2^30, IC, OC <= 2^22 (OC of a gated pair <= 2^21); N * IC, 2 * N * OC and
  *     OC * IC, with IC and OC rounded up to 8, below 2^34. Any other size, any stride, pointers aligned to their element.
  *     Large bf16 products copy operands whose row length or stride is no multiple of 8 elements, or whose address is no
- *     multiple of 16 bytes, into the workspace; all others are read in place. A bf16 element is read with the 4-byte word
+ *     multiple of 16 bytes, and fp32 pairs of filters of two strides, into the workspace; all others are read in place. A bf16 element is read with the 4-byte word
  *     it lies in.
  *   - N, IC and OC may be 0: an empty sum is 0 (IC = 0: Z = Bias; N = 0: deltaW and deltaB are zeros).
  *   - All pointers are DEVICE pointers, borrowed for the duration of the enqueued work. Nothing is allocated, freed or
