@@ -13,8 +13,8 @@
  *     in elements (>= the row's length, <= 2^22). N < 2^30, IC, OC <= 2^22 (OC of a gated pair <= 2^21); N * IC, 2 * N * OC and
  *     OC * IC, with IC and OC rounded up to 8, below 2^34. Any other size, any stride, pointers aligned to their element.
  *     Large bf16 products copy operands whose row length or stride is no multiple of 8 elements, or whose address is no
- *     multiple of 16 bytes, and fp32 pairs of filters of two strides, into the workspace; all others are read in place. A bf16 element is read with the 4-byte word
- *     it lies in.
+ *     multiple of 16 bytes, and a pair of filters of two strides may be copied, into the workspace; all others are read in
+ *     place. A bf16 element is read with the 4-byte word it lies in.
  *   - N, IC and OC may be 0: an empty sum is 0 (IC = 0: Z = Bias; N = 0: deltaW and deltaB are zeros).
  *   - All pointers are DEVICE pointers, borrowed for the duration of the enqueued work. Nothing is allocated, freed or
  *     synchronised; scratch is supplied by the caller: alpha_*_workspace gives its bytes for a call's type and sizes (0 to 2^63-1,
@@ -24,10 +24,11 @@
  *   - `streams`, `length`: as in alpha_conv.h; everything is enqueued on streams[0], which belongs to the current device,
  *     as does the memory. Calls may be captured into a graph. Results are bit-identical from run to run.
  *   - Outputs must not overlap inputs, the workspace or each other, except where said.
- *   - Large fp32 products run on the bf16 matrix pipe as sums of three-part splits: six of the nine partial products, the left-out
- *     ones together below 2^-23 of a product. The split keeps all 24 bits of an operand of 2^-110 and more; of a smaller one, whose
- *     last parts would be below bf16's last subnormal, it keeps what is above 2^-134. Others are plain fp32. Infinities and NaN come out as in
- *     plain fp32 either way; what is not finite is computed again, so a product that is full of them takes three to four times as long.
+ *   - Large fp32 products run on the bf16 matrix pipe as sums of three-part splits: six of the nine partial products, the
+ *     left-out ones together below 2^-23 of a product. The split keeps all 24 bits of an operand of 2^-110 and more; of a
+ *     smaller one, whose last parts would be below bf16's last subnormal, it keeps what is above 2^-134. Others are plain
+ *     fp32. Infinities and NaN come out as in plain fp32 either way; what is not finite is computed again, so a product that is
+ *     full of them takes three to four times as long.
  *
  * Return value: 0 on success, a hipError_t value, or ALPHA_DENSE_EINVAL; alpha_dense_last_error() has the thread's message.
  */
@@ -99,9 +100,10 @@ int alpha_dgatedMatMul(const int64_t *streams, int length, int type,
 /* The global norm of `count` gradients and clipping by it:
  *     norm = sqrt(sum over all tensors and elements of g^2),  c = min(1, max_norm / (norm + eps)),  dst = g * c.
  * types[i], lengths[i] (elements, >= 0), src[i], dst[i]: HOST arrays, read during the call; the tensors are dense device
- * memory aligned to their element, dst[i] of src[i]'s type, and dst[i] may be src[i] (in place) but no other src or dst: the same gradient
- * twice is refused where it would be scaled twice. dst may be NULL: only the norm. norm_c: two device floats, {norm, c}, written; NaN and infinities follow the formula (a NaN makes c NaN; an
- * infinite norm makes c 0 and the infinite elements NaN), so a caller sees them in norm_c[0]. max_norm and eps are finite and >= 0, max_norm + eps > 0. */
+ * memory aligned to their element, dst[i] of src[i]'s type, and dst[i] may be src[i] (in place) but no other src or dst: the
+ * same gradient twice is refused where it would be scaled twice. dst may be NULL: only the norm. norm_c: two device floats,
+ * {norm, c}, written; NaN and infinities follow the formula (a NaN makes c NaN; an infinite norm makes c 0 and the infinite
+ * elements NaN), so a caller sees them in norm_c[0]. max_norm and eps are finite and >= 0, max_norm + eps > 0. */
 int64_t alpha_gradClip_workspace(int count, const int64_t *lengths);
 int alpha_gradClip(const int64_t *streams, int length, int count, const int *types, const int64_t *lengths,
                    const void *const *src, void *const *dst, float max_norm, float eps, float *norm_c,

@@ -84,7 +84,7 @@ BACKWARD = [
     ("bf16", 5000, 2001, 5001, ("st", 256, 256, False), ("tt", 256, 256, False)),
 ]
 GATED_BACKWARD = [
-    ("f32", 245, 1497, 625, ("st", 128, 128, True)), ("f32", 133, 301, 4483, ("tt", 128, 128, False)), ("f32", 2489, 71, 1797, ("tt", 128, 128, True)),
+    ("f32", 3587, 2995, 39, ("st", 128, 128, False)), ("f32", 245, 1497, 625, ("st", 128, 128, True)), ("f32", 133, 301, 4483, ("tt", 128, 128, False)), ("f32", 2489, 71, 1797, ("tt", 128, 128, True)),
     ("f32", 2149, 491, 4585, ("st", 256, 128, True)), ("f32", 2001, 515, 2001, ("tt", 256, 128, True)), ("f32", 75, 1841, 1177, ("tt", 256, 128, False)),
     ("bf16", 1500, 777, 1300, ("st", 128, 128, True)), ("bf16", 2481, 599, 3875, ("st", 256, 128, True)), ("bf16", 4873, 2199, 311, ("st", 256, 256, False)),
     ("bf16", 678, 3609, 4841, ("st", 256, 256, True)), ("bf16", 4001, 24, 4007, ("tt", 128, 128, True)), ("bf16", 851, 673, 2753, ("tt", 256, 128, False)),
